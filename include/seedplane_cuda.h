@@ -33,6 +33,10 @@ extern "C" {
 #define SP_ERR_UNSUPPORTED -4   /* shape not supported by the kernels */
 #define SP_ERR_DEVICE      -5   /* a kernel reported an error status (bounded wait, bad index) */
 
+#define SP_F32              0   /* value types of the paged operators and of logits              */
+#define SP_F16              1
+#define SP_BF16             2
+
 #define SP_WEIGHTS_F16       0  /* fp16 matrices (seedplane-bundle/2 layout)                    */
 #define SP_WEIGHTS_I8_B32    1  /* int8 matrices + one fp16 scale per 32 inputs along K          */
 
@@ -225,6 +229,97 @@ int sp_mcol_gemm(sp_engine *e, int32_t mode, const void *w_dev, const void *w_lo
  * top_p in [0, 1], else SP_ERR_INVALID. */
 int sp_sample_filter(const float *logits_dev, int32_t vocab, double temperature, int32_t top_k, double top_p,
                      float *z_dev, void *stream);
+
+/* ---- K / V in pages shared by requests (runtime request batching after a common prefix) --------
+ * No reference counterpart: the reference keeps one contiguous cache per session
+ * (seedplane/qwen_engine.py:18-29) and decodes requests one at a time (README.md:67-68).
+ *
+ * One layer's pages. K (and V) of kv head g at slot j of page p is the head_dim elements at
+ * p * page_stride + g * head_stride + j * slot_stride (elements; multiples of 8, and k_dev, v_dev
+ * 16-byte aligned). head_dim 64 or 128, dtype SP_F16 or SP_BF16, any page_size >= 1.
+ * status_dev: int32 on the device, or NULL. A kernel that meets a bad page number, length or
+ * position stores 3 there (slots it cannot reach are not written, and read as absent) and goes on. */
+typedef struct sp_pages {
+    void *k_dev, *v_dev;
+    int64_t page_stride, head_stride, slot_stride;
+    int32_t n_pages, page_size, kv_heads, head_dim, dtype;
+    int32_t *status_dev;
+} sp_pages;
+
+/* A ragged batch over pages. Request b's tokens of this call are the rows q_start[b] ..
+ * q_start[b + 1] - 1 of the call's matrices (q_start int32 [batch + 1], q_start[0] = 0; NULL: max_q
+ * rows each; a request may have none). lens[b]: its own keys, these tokens among them, which are the
+ * last: token i has own key lens[b] - q_len + i. Own key j is slot j % page_size of page
+ * tables[b * table_stride + j / page_size]. Before its own keys every request sees the shared prefix:
+ * keys [0, prefix_len) in the pages of prefix_dev, in order. The arrays are device memory and are read
+ * by the kernels, so a captured graph serves new contents; the sizes are the host's: `tokens` rows at
+ * most (rows at and behind q_start[batch] are neither read nor written), max_q rows of one request at
+ * most. */
+typedef struct sp_page_batch {
+    int32_t batch, tokens, max_q;
+    const int32_t *q_start_dev, *lens_dev, *tables_dev;
+    int64_t table_stride;
+    int32_t table_width;
+    const int32_t *prefix_dev;
+    int32_t prefix_len;
+} sp_page_batch;
+
+/* Append a pass's keys and values to their pages with the position rotation on the way. x =
+ * qkv row + bias (bias fp32 [(heads + 2 kv_heads) * head_dim] or NULL); row = q heads, then k, then v
+ * (the fused QKV order of sp_layer_weights), row_stride elements apart. Of every q and k head the
+ * first rot_dim dims (even, <= head_dim) are rotated in pairs (a, b) -> (a c - b s, b c + a s), pairs
+ * (j, j + rot_dim / 2) or, `interleaved`, (2j, 2j + 1); (c, s) = rope_dev[pos][j], fp32
+ * [rope_positions][rot_dim / 2][2] (sp_weights.rope_host's layout; a scaled table gives scaled
+ * positions). pos = positions_dev[row], or prefix_len + own key when NULL. q goes to q_out [row][heads
+ * * head_dim] (q_stride elements apart) in the rows' type; k and v are rounded to the cache's type.
+ * dtype: SP_F32 (either cache type), or the cache's own type. All arithmetic is fp32. `device`: the
+ * device of every pointer; the calling thread's current device is put back. Nothing is allocated;
+ * the call can be captured into a graph. */
+int sp_pages_append(int device, const sp_pages *pages, const sp_page_batch *batch, int32_t heads, const void *qkv_dev,
+                    int32_t dtype, int64_t row_stride, const float *bias_dev, const float *rope_dev,
+                    int32_t rope_positions, int32_t rot_dim, int32_t interleaved, const int32_t *positions_dev,
+                    void *q_out_dev, int64_t q_stride, void *stream);
+
+/* Bytes of workspace sp_pages_attention needs for these sizes (0 is possible), or SP_ERR_*. */
+int64_t sp_pages_attention_workspace(const sp_pages *pages, const sp_page_batch *batch, int32_t heads, int32_t dtype);
+
+/* Attention of a batch whose requests share a prefix: out[row] = softmax(scale * q . K) V over the
+ * prefix's keys and the request's own keys up to the row's own; the prefix's pages are read once for
+ * the whole batch. q, out: [row][heads * head_dim], q_stride / out_stride elements apart (multiples of
+ * 8, 16-byte aligned). dtype of q and out: SP_F32 over SP_F16 pages (scores and values then carry the
+ * queries and probabilities as two fp16 halves, ~22 bits), or the pages' own type (probabilities
+ * rounded to it; sums, maxima and outputs fp32, rounded once). A row that sees no key gives zeros.
+ * lse_dev: NULL or fp32 [row][heads], the log-sum-exp of the scaled scores (-inf for such a row).
+ * workspace_dev: as many bytes as sp_pages_attention_workspace says, 16-byte aligned, contents free,
+ * not shared by calls that may overlap in time. Can be captured into a graph. */
+int sp_pages_attention(int device, const sp_pages *pages, const sp_page_batch *batch, int32_t heads, const void *q_dev,
+                       int32_t dtype, int64_t q_stride, float scale, void *out_dev, int64_t out_stride, float *lse_dev,
+                       void *workspace_dev, int64_t workspace_bytes, void *stream);
+
+/* Bytes of workspace sp_accept_chains needs, or SP_ERR_*. */
+int64_t sp_accept_chains_workspace(int32_t batch, int32_t drafts, int32_t vocab);
+
+/* Verification of every request's chain of drafted tokens with given random numbers, a whole batch in
+ * one call and without a synchronisation (sp_accept_stochastic: one request's tree, its own random
+ * numbers, on the host's time; the reference verifies greedily, seedplane/speculative.py:55-92).
+ * Request b drafted tokens_dev[b][0 .. n), n = counts_dev[b] (NULL: all `drafts`). With p_i =
+ * softmax(target row i / T_b) and q_i = softmax(draft row i / T_b) (draft_dev NULL: the drafter is
+ * certain, q_i = 1 at its token), draft i is accepted when u[b][i] * q_i(x_i) < p_i(x_i). After the
+ * first refusal i the next token is drawn from max(p_i - q_i, 0), or from p_i where that is zero
+ * everywhere; after n acceptances from p_n. A draw from weights r is the first index whose running
+ * sum exceeds u[b][drafts] * (their sum). T_b = temperature_dev[b] (fp32; NULL: 1); T_b <= 0: greedy,
+ * p_i is 1 at the row's first maximum. NaN logits weigh nothing; a row without a finite or +inf logit
+ * accepts nothing and draws -1; a drafted token outside [0, vocab) is refused.
+ * target_dev: [b][drafts + 1][vocab], rows target_ld and requests target_bs elements apart; draft_dev:
+ * [b][drafts][vocab], draft_ld, draft_bs; dtype SP_F32, SP_F16 or SP_BF16; u_dev fp64 [b][drafts + 1] in
+ * [0, 1). out_tokens_dev int32 [b][drafts + 1]: the accepted tokens, the drawn one, then -1;
+ * accepted_dev int32 [b]. drafts 0 .. 64 (0: a draw for every request). Probabilities and sums are
+ * fp64. workspace_dev as above. */
+int sp_accept_chains(int device, int32_t batch, int32_t drafts, int32_t vocab, const void *target_dev, int64_t target_bs,
+                     int64_t target_ld, const void *draft_dev, int64_t draft_bs, int64_t draft_ld, int32_t dtype,
+                     const int32_t *tokens_dev, const int32_t *counts_dev, const double *u_dev,
+                     const float *temperature_dev, int32_t *out_tokens_dev, int32_t *accepted_dev, void *workspace_dev,
+                     int64_t workspace_bytes, void *stream);
 
 /* sp_argmax without an engine and without any allocation (no reference counterpart: the
  * reference allocates nothing on this path; this entry point exists for callers that must not

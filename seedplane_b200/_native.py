@@ -15,6 +15,9 @@ SP_ERR_CUDA = -2
 SP_ERR_CAPACITY = -3
 SP_ERR_UNSUPPORTED = -4
 SP_ERR_DEVICE = -5
+SP_F32 = 0
+SP_F16 = 1
+SP_BF16 = 2
 SP_WEIGHTS_F16 = 0
 SP_WEIGHTS_I8_B32 = 1
 
@@ -23,6 +26,8 @@ EXPORTED = ("sp_last_error", "sp_version", "sp_engine_create", "sp_engine_destro
             "sp_kv_create", "sp_kv_destroy", "sp_kv_length", "sp_kv_capacity", "sp_kv_set_length",
             "sp_forward", "sp_decode", "sp_decode_batch", "sp_prefill_batch", "sp_verify_tree", "sp_kv_commit", "sp_kv_copy", "sp_argmax", "sp_argmax_noalloc", "sp_mcol_gemm", "sp_topk",
             "sp_accept_stochastic", "sp_accept_greedy", "sp_sample_filter",
+            "sp_pages_append", "sp_pages_attention", "sp_pages_attention_workspace",
+            "sp_accept_chains", "sp_accept_chains_workspace",
             "sp_device_status",
             "sp_trace_read")
 
@@ -46,6 +51,20 @@ class SpLayerWeights(C.Structure):
 class SpWeights(C.Structure):
     _fields_ = [("embed", C.c_void_p), ("lm_head", C.c_void_p), ("lm_head_s", C.c_void_p),
                 ("final_norm", C.c_void_p), ("layers", C.POINTER(SpLayerWeights)), ("rope_host", C.c_void_p)]
+
+
+class SpPages(C.Structure):
+    _fields_ = [("k_dev", C.c_void_p), ("v_dev", C.c_void_p),
+                ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("slot_stride", C.c_int64),
+                ("n_pages", C.c_int32), ("page_size", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("dtype", C.c_int32), ("status_dev", C.c_void_p)]
+
+
+class SpPageBatch(C.Structure):
+    _fields_ = [("batch", C.c_int32), ("tokens", C.c_int32), ("max_q", C.c_int32),
+                ("q_start_dev", C.c_void_p), ("lens_dev", C.c_void_p), ("tables_dev", C.c_void_p),
+                ("table_stride", C.c_int64), ("table_width", C.c_int32),
+                ("prefix_dev", C.c_void_p), ("prefix_len", C.c_int32)]
 
 
 _lib = None
@@ -87,6 +106,14 @@ def load(path: Path = LIB_PATH):
                                            C.c_uint64, pi32, vp]),
         "sp_accept_greedy": (C.c_int, [vp, vp, i32, pi32, pi32, i32, pi32, i32, pi32, vp]),
         "sp_sample_filter": (C.c_int, [vp, i32, C.c_double, i32, C.c_double, vp, vp]),
+        "sp_pages_append": (C.c_int, [C.c_int, C.POINTER(SpPages), C.POINTER(SpPageBatch), i32, vp, i32, i64, vp, vp,
+                                      i32, i32, i32, vp, vp, i64, vp]),
+        "sp_pages_attention_workspace": (i64, [C.POINTER(SpPages), C.POINTER(SpPageBatch), i32, i32]),
+        "sp_pages_attention": (C.c_int, [C.c_int, C.POINTER(SpPages), C.POINTER(SpPageBatch), i32, vp, i32, i64,
+                                         C.c_float, vp, i64, vp, vp, i64, vp]),
+        "sp_accept_chains_workspace": (i64, [i32, i32, i32]),
+        "sp_accept_chains": (C.c_int, [C.c_int, i32, i32, i32, vp, i64, i64, vp, i64, i64, i32, vp, vp, vp, vp, vp, vp,
+                                       vp, i64, vp]),
         "sp_device_status": (C.c_int, [vp, vp]),
         "sp_trace_read": (i64, [vp, C.POINTER(C.c_uint64), i64]),
     }

@@ -1805,6 +1805,182 @@ int sp_accept_greedy(sp_engine *e, const int32_t *node_pred_dev, int32_t root_pr
     return SP_OK;
 }
 
+// ---- paged operators ---------------------------------------------------------------------------
+namespace {
+// the caller's current device is put back on every return
+struct OnDevice {
+    int prev = -1;
+    cudaError_t enter(int device) {
+        int cur = -1;
+        cudaError_t e = cudaGetDevice(&cur);
+        if (e != cudaSuccess || cur == device) return e;
+        e = cudaSetDevice(device);
+        if (e == cudaSuccess) prev = cur;
+        return e;
+    }
+    ~OnDevice() { if (prev >= 0) cudaSetDevice(prev); }
+};
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+int check_pages(const sp_pages *pages, const sp_page_batch *batch, int32_t heads, PagesView &pg, PageBatchView &ba) {
+    if (!pages || !batch) return fail(SP_ERR_INVALID, "null argument");
+    if (pages->head_dim != 64 && pages->head_dim != 128)
+        return fail(SP_ERR_UNSUPPORTED, "pages: head_dim %d (64 or 128)", pages->head_dim);
+    if (pages->dtype != SP_F16 && pages->dtype != SP_BF16)
+        return fail(SP_ERR_UNSUPPORTED, "pages: dtype %d (SP_F16 or SP_BF16)", pages->dtype);
+    if (pages->n_pages < 0 || pages->page_size < 1 || pages->kv_heads < 1 || pages->kv_heads > 65535)
+        return fail(SP_ERR_INVALID, "pages: %d pages of %d slots, %d kv heads", pages->n_pages, pages->page_size,
+                    pages->kv_heads);
+    if (heads < 1 || heads % pages->kv_heads)
+        return fail(SP_ERR_INVALID, "%d heads are not a multiple of %d kv heads", heads, pages->kv_heads);
+    if (pages->n_pages > 0 && (!pages->k_dev || !pages->v_dev)) return fail(SP_ERR_INVALID, "pages: null K or V");
+    if (!aligned16(pages->k_dev) || !aligned16(pages->v_dev) || pages->page_stride % 8 || pages->head_stride % 8 ||
+        pages->slot_stride % 8)
+        return fail(SP_ERR_INVALID, "pages: K and V must be 16-byte aligned, with strides that are multiples of 8");
+    if (batch->batch < 0 || batch->tokens < 0 || batch->max_q < 0 || batch->prefix_len < 0 || batch->table_width < 0)
+        return fail(SP_ERR_INVALID, "batch: a negative size");
+    if (batch->tokens > 0 && (batch->batch < 1 || batch->max_q < 1 || !batch->lens_dev))
+        return fail(SP_ERR_INVALID, "batch: %d rows of %d requests, max_q %d, %s", batch->tokens, batch->batch, batch->max_q,
+                    batch->lens_dev ? "lens" : "no lens");
+    if (batch->table_width > 0 && (!batch->tables_dev || batch->table_stride < batch->table_width))
+        return fail(SP_ERR_INVALID, "batch: %s, rows %lld apart for %d pages", batch->tables_dev ? "tables" : "no tables",
+                    (long long)batch->table_stride, batch->table_width);
+    if (batch->prefix_len > 0 && !batch->prefix_dev) return fail(SP_ERR_INVALID, "batch: prefix without pages");
+    if (pages->n_pages == 0 && (batch->prefix_len > 0 || batch->table_width > 0))
+        return fail(SP_ERR_INVALID, "batch: tables into no pages");
+    // key numbers, and positions behind the prefix, are 32-bit
+    if ((int64_t)batch->prefix_len + (int64_t)batch->table_width * pages->page_size > INT32_MAX - 4096 ||
+        (int64_t)batch->tokens * heads > INT32_MAX / 2)
+        return fail(SP_ERR_CAPACITY, "batch: more keys or rows than 32-bit numbers count");
+    pg = PagesView{pages->k_dev, pages->v_dev, pages->page_stride, pages->head_stride, pages->slot_stride,
+                   pages->n_pages, pages->page_size, pages->kv_heads, pages->head_dim, pages->status_dev};
+    ba = PageBatchView{batch->batch, batch->tokens, batch->max_q, batch->q_start_dev, batch->lens_dev, batch->tables_dev,
+                       batch->table_stride, batch->table_width, batch->prefix_dev, batch->prefix_len};
+    return SP_OK;
+}
+
+int attention_args(const sp_pages *pages, const sp_page_batch *batch, int32_t heads, int32_t dtype, PagesAttention &p) {
+    int rc = check_pages(pages, batch, heads, p.pg, p.ba);
+    if (rc) return rc;
+    if (!(dtype == pages->dtype || (dtype == SP_F32 && pages->dtype == SP_F16)))
+        return fail(SP_ERR_UNSUPPORTED, "queries of dtype %d over pages of dtype %d", dtype, pages->dtype);
+    p.nh = heads;
+    p.q_type = dtype;
+    p.cache_type = pages->dtype;
+    return SP_OK;
+}
+}  // namespace
+
+int sp_pages_append(int device, const sp_pages *pages, const sp_page_batch *batch, int32_t heads, const void *qkv_dev,
+                    int32_t dtype, int64_t row_stride, const float *bias_dev, const float *rope_dev,
+                    int32_t rope_positions, int32_t rot_dim, int32_t interleaved, const int32_t *positions_dev,
+                    void *q_out_dev, int64_t q_stride, void *stream) {
+    PagesAppend p{};
+    int rc = check_pages(pages, batch, heads, p.pg, p.ba);
+    if (rc) return rc;
+    if (dtype != SP_F32 && dtype != pages->dtype)
+        return fail(SP_ERR_UNSUPPORTED, "rows of dtype %d into pages of dtype %d", dtype, pages->dtype);
+    if (p.ba.T == 0) return SP_OK;
+    const int64_t q_cols = (int64_t)heads * pages->head_dim, cols = q_cols + 2ll * pages->kv_heads * pages->head_dim;
+    if (!qkv_dev || !q_out_dev || !rope_dev) return fail(SP_ERR_INVALID, "null argument");
+    if (row_stride < cols || q_stride < q_cols)
+        return fail(SP_ERR_INVALID, "rows %lld apart for %lld values, q rows %lld for %lld", (long long)row_stride,
+                    (long long)cols, (long long)q_stride, (long long)q_cols);
+    if (rot_dim < 2 || rot_dim % 2 || rot_dim > pages->head_dim || rope_positions < 1)
+        return fail(SP_ERR_INVALID, "rot_dim %d (even, 2..%d), %d positions", rot_dim, pages->head_dim, rope_positions);
+    p.nh = heads;
+    p.in_type = dtype;
+    p.cache_type = pages->dtype;
+    p.x = qkv_dev;
+    p.x_stride = row_stride;
+    p.bias = bias_dev;
+    p.rope = rope_dev;
+    p.rope_positions = rope_positions;
+    p.rot = rot_dim;
+    p.interleaved = interleaved != 0;
+    p.pos = positions_dev;
+    p.q = q_out_dev;
+    p.q_stride = q_stride;
+    OnDevice on;
+    SP_CUDA(on.enter(device));
+    SP_CUDA(launch_pages_append(p, (cudaStream_t)stream));
+    return SP_OK;
+}
+
+int64_t sp_pages_attention_workspace(const sp_pages *pages, const sp_page_batch *batch, int32_t heads, int32_t dtype) {
+    PagesAttention p{};
+    int rc = attention_args(pages, batch, heads, dtype, p);
+    return rc ? rc : p.ba.T == 0 ? 0 : (int64_t)pages_attention_workspace(p);
+}
+
+int sp_pages_attention(int device, const sp_pages *pages, const sp_page_batch *batch, int32_t heads, const void *q_dev,
+                       int32_t dtype, int64_t q_stride, float scale, void *out_dev, int64_t out_stride, float *lse_dev,
+                       void *workspace_dev, int64_t workspace_bytes, void *stream) {
+    PagesAttention p{};
+    int rc = attention_args(pages, batch, heads, dtype, p);
+    if (rc) return rc;
+    if (p.ba.T == 0) return SP_OK;
+    const int64_t cols = (int64_t)heads * pages->head_dim;
+    if (!q_dev || !out_dev) return fail(SP_ERR_INVALID, "null argument");
+    if (q_stride < cols || out_stride < cols || q_stride % 8 || out_stride % 8 || !aligned16(q_dev) || !aligned16(out_dev))
+        return fail(SP_ERR_INVALID, "q and out: 16-byte aligned rows of %lld values, strides that are multiples of 8",
+                    (long long)cols);
+    if (!(scale > 0.f) || !std::isfinite(scale)) return fail(SP_ERR_INVALID, "scale must be positive and finite");
+    const int64_t need = (int64_t)pages_attention_workspace(p);
+    if (workspace_bytes < need || (need > 0 && (!workspace_dev || !aligned16(workspace_dev))))
+        return fail(SP_ERR_INVALID, "workspace of %lld bytes, %lld needed, 16-byte aligned", (long long)workspace_bytes,
+                    (long long)need);
+    p.q = q_dev;
+    p.q_stride = q_stride;
+    p.scale = scale;
+    p.out = out_dev;
+    p.out_stride = out_stride;
+    p.lse = lse_dev;
+    p.ws = workspace_dev;
+    OnDevice on;
+    SP_CUDA(on.enter(device));
+    SP_CUDA(launch_pages_attention(p, (cudaStream_t)stream));
+    return SP_OK;
+}
+
+static int check_chains(int32_t batch, int32_t drafts, int32_t vocab) {
+    if (batch < 0 || vocab < 1) return fail(SP_ERR_INVALID, "%d requests, vocab %d", batch, vocab);
+    if (drafts < 0 || drafts > kChainMaxDrafts) return fail(SP_ERR_CAPACITY, "%d drafts (0..%d)", drafts, kChainMaxDrafts);
+    if (vocab > INT32_MAX - 65536 || (int64_t)batch * (2 * drafts + 1) * ((int64_t)vocab / 1024 + 1) > INT32_MAX)
+        return fail(SP_ERR_CAPACITY, "%d requests of %d drafts over %d logits are too many", batch, drafts, vocab);
+    return SP_OK;
+}
+
+int64_t sp_accept_chains_workspace(int32_t batch, int32_t drafts, int32_t vocab) {
+    int rc = check_chains(batch, drafts, vocab);
+    return rc ? rc : (int64_t)chains_workspace(batch, drafts, vocab);
+}
+
+int sp_accept_chains(int device, int32_t batch, int32_t drafts, int32_t vocab, const void *target_dev, int64_t target_bs,
+                     int64_t target_ld, const void *draft_dev, int64_t draft_bs, int64_t draft_ld, int32_t dtype,
+                     const int32_t *tokens_dev, const int32_t *counts_dev, const double *u_dev,
+                     const float *temperature_dev, int32_t *out_tokens_dev, int32_t *accepted_dev, void *workspace_dev,
+                     int64_t workspace_bytes, void *stream) {
+    int rc = check_chains(batch, drafts, vocab);
+    if (rc) return rc;
+    if (dtype != SP_F32 && dtype != SP_F16 && dtype != SP_BF16) return fail(SP_ERR_UNSUPPORTED, "logits of dtype %d", dtype);
+    if (batch == 0) return SP_OK;
+    if (!target_dev || !u_dev || !out_tokens_dev || !accepted_dev || (drafts > 0 && !tokens_dev))
+        return fail(SP_ERR_INVALID, "null argument");
+    if (target_ld < vocab || (draft_dev && drafts > 0 && draft_ld < vocab) || target_bs < 0 || draft_bs < 0)
+        return fail(SP_ERR_INVALID, "bad logits shape");
+    const int64_t need = (int64_t)chains_workspace(batch, drafts, vocab);
+    if (workspace_bytes < need || !workspace_dev || !aligned16(workspace_dev))
+        return fail(SP_ERR_INVALID, "workspace of %lld bytes, %lld needed, 16-byte aligned", (long long)workspace_bytes,
+                    (long long)need);
+    ChainArgs a{batch, drafts, vocab, dtype, target_dev, drafts > 0 ? draft_dev : nullptr, target_bs, target_ld, draft_bs,
+                draft_ld, tokens_dev, counts_dev, u_dev, temperature_dev, out_tokens_dev, accepted_dev, workspace_dev};
+    OnDevice on;
+    SP_CUDA(on.enter(device));
+    SP_CUDA(launch_accept_chains(a, (cudaStream_t)stream));
+    return SP_OK;
+}
+
 int sp_argmax_noalloc(int device, const float *logits_dev, int32_t rows, int32_t cols, int64_t ld, int32_t *argmax_dev,
                       void *stream) {
     if (!logits_dev || !argmax_dev) return fail(SP_ERR_INVALID, "null logits or output");

@@ -443,6 +443,69 @@ constexpr int kGreedyMaxPaths = 1024;
 cudaError_t launch_accept_greedy(const int *pred, int root_pred, const int *tok, const int *parent, int n,
                                  const int *ends, int n_paths, int *out, cudaStream_t s);
 
+// ---- K / V in pages: pages.cu -------------------------------------------------------------------
+// One layer's pages and a ragged batch over them, as sp_pages and sp_page_batch describe them.
+constexpr int kErrPages = 3;                 // stored at `status` (= kErrBadSlot)
+struct PagesView {
+    void *k, *v;
+    long long page_stride, head_stride, slot_stride;
+    int n_pages, page_size, nkv, hd;
+    int *status;
+};
+struct PageBatchView {
+    int B, T, max_q;
+    const int *q_start, *lens, *tables;
+    long long table_stride;
+    int table_width;
+    const int *prefix;
+    int prefix_len;
+};
+enum ValueType : int { VT_F32 = 0, VT_F16 = 1, VT_BF16 = 2 };
+struct PagesAppend {
+    PagesView pg;
+    PageBatchView ba;
+    int nh, in_type, cache_type;
+    const void *x;
+    long long x_stride;
+    const float *bias, *rope;
+    int rope_positions, rot, interleaved;
+    int paired;              // rows with RoPE partners adjacent (the batched pass's packed QKV rows):
+                             // row element h hd + 2 d + e is dim d + e hd / 2 of head h
+    const int *pos;
+    void *q;
+    long long q_stride;
+};
+cudaError_t launch_pages_append(const PagesAppend &p, cudaStream_t s);
+struct PagesAttention {
+    PagesView pg;
+    PageBatchView ba;
+    int nh, q_type, cache_type;
+    const void *q;
+    long long q_stride;
+    float scale;
+    void *out;
+    long long out_stride;
+    float *lse;
+    void *ws;
+};
+size_t pages_attention_workspace(const PagesAttention &p);
+cudaError_t launch_pages_attention(const PagesAttention &p, cudaStream_t s);
+
+// Verification of a batch's draft chains (chains.cu), as sp_accept_chains describes it.
+constexpr int kChainMaxDrafts = 64;
+struct ChainArgs {
+    int B, n, V, type;
+    const void *target, *draft;
+    long long target_bs, target_ld, draft_bs, draft_ld;
+    const int *tokens, *counts;
+    const double *u;
+    const float *temperature;
+    int *out_tokens, *accepted;
+    void *ws;
+};
+size_t chains_workspace(int B, int n, int V);
+cudaError_t launch_accept_chains(const ChainArgs &a, cudaStream_t s);
+
 // Row-wise greedy argmax (argmax.cu). A row is split over argmax_ctas(cols) CTAs whose partial
 // (max, index) pairs meet in the scratch: val / idx [rows][kArgmaxMaxCtas] and one counter per
 // row, which must be zero when the kernel starts and is zero again when it ends.

@@ -1,0 +1,136 @@
+// Device helpers of the paged operators (pages.cu): value types, the ragged batch, pages and key
+// ranges.
+#pragma once
+
+#include <atomic>
+#include <type_traits>
+
+#include <cuda_bf16.h>
+
+#include "kernels.cuh"
+
+namespace sp {
+
+// ---- value types -------------------------------------------------------------------------------
+SP_DEVINL float to_float(float v) { return v; }
+SP_DEVINL float to_float(__half v) { return __half2float(v); }
+SP_DEVINL float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+SP_DEVINL T from_float(float v) {
+    if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __float2bfloat16_rn(v);
+    else return v;
+}
+// two values as one 32-bit word, a in the low half
+template <typename T>
+SP_DEVINL uint32_t pack2(float a, float b) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+template <typename T>
+SP_DEVINL void unpack2(uint32_t w, float &a, float &b) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+        a = f.x;
+        b = f.y;
+    } else {
+        a = __uint_as_float(w << 16);
+        b = __uint_as_float(w & 0xffff0000u);
+    }
+}
+SP_DEVINL float exp2_approx(float x) {                       // 2^x, relative error below 2^-22; 2^-inf = 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// log-sum-exp of a row from its base-2 maximum and sum
+SP_DEVINL float row_lse(float m, float l) {
+    return m == -INFINITY ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+// ---- the ragged batch --------------------------------------------------------------------------
+SP_DEVINL void set_status(int *status) {
+    if (status) atomicCAS(status, 0, kErrPages);
+}
+SP_DEVINL int request_start(const PageBatchView &ba, int b) {
+    return ba.q_start ? min(max(ba.q_start[b], 0), ba.T) : (int)min((long long)b * ba.max_q, (long long)ba.T);
+}
+// rows of the call: q_start's last, within the host's bound
+SP_DEVINL int total_rows(const PageBatchView &ba) {
+    return ba.q_start ? min(ba.T, ba.q_start[ba.B]) : (int)min((long long)ba.T, (long long)ba.B * ba.max_q);
+}
+// The request of row t < q_start[B] (the last b with q_start[b] <= t), by the whole warp: 32 probes a
+// round.
+SP_DEVINL int find_request(const PageBatchView &ba, int t, int lane) {
+    if (!ba.q_start) return t / ba.max_q;
+    int lo = 0, n = ba.B;
+    while (n > 1) {
+        const int step = (n + 31) / 32, at = lane * step;
+        const bool le = at < n && ba.q_start[lo + at] <= t;
+        const int c = max(0, __popc(__ballot_sync(0xffffffffu, le)) - 1) * step;
+        lo += c;
+        n = min(step, n - c);
+    }
+    return lo;
+}
+// a request's own keys, within its table
+SP_DEVINL int own_len(const PagesAttention &p, int b, int lane) {
+    const int len = p.ba.lens[b];
+    const long long cap = (long long)p.ba.table_width * p.pg.page_size;
+    if (len < 0 || len > cap) {
+        if (lane == 0) set_status(p.pg.status);
+        return len < 0 ? 0 : (int)cap;
+    }
+    return len;
+}
+// element offset of a key's row in its page, -1 on a bad page number
+SP_DEVINL long long page_row(const PagesView &pg, const int *table, int key) {
+    const int pi = key / pg.page_size, page = table[pi];
+    if ((unsigned)page >= (unsigned)pg.n_pages) {
+        set_status(pg.status);
+        return -1;
+    }
+    return (long long)page * pg.page_stride + (long long)(key - pi * pg.page_size) * pg.slot_stride;
+}
+
+// ---- key ranges --------------------------------------------------------------------------------
+constexpr int kPagesGrain = 128;                             // key ranges are multiples of this
+constexpr int kPagesOwnKeys = 256;                           // own keys per range at least
+constexpr int kPagesMaxSplits = 32;
+struct PagesPlan {
+    int prefix_tiles, prefix_splits, prefix_chunk;           // row tiles of the whole batch x key ranges
+    int own_tiles, own_splits;                               // row tiles of a request x key ranges at most
+    int slots;                                               // partials per (token, head); 1: no merge
+    float *acc, *ml;                                         // [slots][T][heads][hd], [slots][T][heads][m, l]
+};
+// a request's own keys in at most `most` ranges of `chunk` keys (the same in every kernel)
+SP_DEVINL void own_chunks(int len, int most, int &chunk, int &n) {
+    const int want = max(1, min(most, (len + kPagesOwnKeys - 1) / kPagesOwnKeys));
+    chunk = max(kPagesGrain, ((len + want - 1) / want + kPagesGrain - 1) / kPagesGrain * kPagesGrain);
+    n = max(1, (len + chunk - 1) / chunk);                   // no key: one empty range
+}
+
+// Raise a kernel's dynamic shared memory limit, once per device and kernel.
+template <typename... KArgs>
+cudaError_t raise_smem(void (*kernel)(KArgs...), int bytes) {
+    static std::atomic<const void *> done[64][32];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    for (int i = 0; i < 32; ++i)
+        if (done[dev & 63][i].load() == reinterpret_cast<const void *>(kernel)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+    for (int i = 0; i < 32; ++i) {
+        const void *none = nullptr;
+        if (done[dev & 63][i].compare_exchange_strong(none, reinterpret_cast<const void *>(kernel))) break;
+    }
+    return cudaSuccess;
+}
+
+}  // namespace sp

@@ -262,6 +262,55 @@ def accept_stochastic(engine, flat: FlatForest, target_logits, draft_logits, tem
     return Verification(emitted, n_acc, n_out > n_acc, n_out, path), nodes
 
 
+def accept_chains(target_logits, draft_logits, drafts, u, *, counts=None, temperature=None, out=None):
+    """Verification of a whole batch's chains of drafted tokens with given random numbers, on the device and
+    without a synchronisation (`sp_accept_chains`; `accept_stochastic` verifies one request's tree with its
+    own counter RNG). target_logits [B, n + 1, V], draft_logits [B, n, V] (None: the drafter is certain of
+    its tokens), fp32, fp16 or bf16; drafts int32 [B, n]; u fp64 [B, n + 1] in [0, 1): column i decides
+    draft i, the last column the draw. counts int32 [B]: drafts per request (None: n). temperature: a number,
+    or fp32 [B]; 0 is greedy. Draft i stays while u_i q_i < p_i; the next token comes from max(p - q, 0) of
+    the first refused row, or from the last row. Returns (tokens int32 [B, n + 1]: the accepted ones, the
+    drawn one, then -1; accepted int32 [B]); `out`: that pair's tensors to write into."""
+    import torch
+    from . import _native as N
+    from .engine import _stream
+    dev = target_logits.device
+    types = {torch.float32: N.SP_F32, torch.float16: N.SP_F16, torch.bfloat16: N.SP_BF16}
+    if target_logits.dim() != 3 or not target_logits.is_cuda or target_logits.dtype not in types or \
+            target_logits.stride(2) != 1:
+        raise ValueError("target_logits: fp32, fp16 or bf16 [B, n + 1, V] on a CUDA device, rows contiguous, expected")
+    B, n1, V = target_logits.shape
+    n = n1 - 1
+    if draft_logits is not None and (draft_logits.shape != (B, n, V) or draft_logits.dtype != target_logits.dtype or
+                                     draft_logits.device != dev or (n > 0 and draft_logits.stride(2) != 1)):
+        raise ValueError(f"draft_logits: [{B}, {n}, {V}] like target_logits expected")
+
+    def need(t, name, dtype, shape):
+        if t.dtype != dtype or t.device != dev or t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"{name}: contiguous {dtype} {list(shape)} on {dev} expected")
+        return t.data_ptr()
+
+    if temperature is not None and not isinstance(temperature, torch.Tensor):
+        temperature = torch.full((B,), float(temperature), dtype=torch.float32, device=dev)
+    if out is None:
+        out = (torch.empty((B, n1), dtype=torch.int32, device=dev), torch.empty(B, dtype=torch.int32, device=dev))
+    lib = N.load()
+    size = lib.sp_accept_chains_workspace(B, n, V)
+    if size < 0:
+        N.check(size)
+    ws = torch.empty(max(1, size), dtype=torch.uint8, device=dev)
+    N.check(lib.sp_accept_chains(
+        dev.index, B, n, V, target_logits.data_ptr(), target_logits.stride(0), target_logits.stride(1),
+        None if draft_logits is None else draft_logits.data_ptr(), 0 if draft_logits is None else draft_logits.stride(0),
+        0 if draft_logits is None else draft_logits.stride(1), types[target_logits.dtype],
+        need(drafts, "drafts", torch.int32, (B, n)), None if counts is None else need(counts, "counts", torch.int32, (B,)),
+        need(u, "u", torch.float64, (B, n1)),
+        None if temperature is None else need(temperature, "temperature", torch.float32, (B,)),
+        need(out[0], "out tokens", torch.int32, (B, n1)), need(out[1], "out accepted", torch.int32, (B,)),
+        ws.data_ptr(), ws.numel(), _stream(dev)))
+    return out
+
+
 def sample_filter(logits_row, temperature: float, top_k: int = 0, top_p: float = 1.0, out=None):
     """The masking of the reference's sample() (qwen_engine.py:147-156) on the device
     (`sp_sample_filter`): z = logits / temperature, -inf where top_k (> 0) or top_p (< 1) drops the
