@@ -238,7 +238,8 @@ int sp_sample_filter(const float *logits_dev, int32_t vocab, double temperature,
  * p * page_stride + g * head_stride + j * slot_stride (elements; multiples of 8, and k_dev, v_dev
  * 16-byte aligned). head_dim 64 or 128, dtype SP_F16 or SP_BF16, any page_size >= 1.
  * status_dev: int32 on the device, or NULL. A kernel that meets a bad page number, length or
- * position stores 3 there (slots it cannot reach are not written, and read as absent) and goes on. */
+ * position stores 3 there (an expired wait inside a kernel: 1) and goes on: slots it cannot reach are not
+ * written, and read as zeros. */
 typedef struct sp_pages {
     void *k_dev, *v_dev;
     int64_t page_stride, head_stride, slot_stride;

@@ -19,7 +19,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 LIB = PKG / "libseedplane_cuda.so"
-SOURCES = ["kernels.cu", "gemv_tc.cu", "attention.cu", "argmax.cu", "step.cu", "prefill.cu", "mcol.cu", "sample.cu", "pages.cu", "chains.cu",
+SOURCES = ["kernels.cu", "gemv_tc.cu", "attention.cu", "argmax.cu", "step.cu", "prefill.cu", "mcol.cu", "sample.cu", "pages.cu", "pages_tc.cu", "chains.cu",
            "engine.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps) k_pages_rows(PagesAttention p
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
     const int g = blockIdx.y, G = p.nh / p.pg.nkv;
     // the item: its rows, its key range and its pages
-    const int n_prefix = pl.prefix_tiles * pl.prefix_splits;
+    const int n_prefix = pl.prefix_tc ? 0 : pl.prefix_tiles * pl.prefix_splits;
     const int total = total_rows(ba);
     int item = blockIdx.x, row0, nrows, q0 = 0, own0 = 0, slot, k_lo, k_hi, k_max;
     const int *table;
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps) k_pages_rows(PagesAttention p
         const int b = item / (pl.own_tiles * pl.own_splits);
         item -= b * pl.own_tiles * pl.own_splits;
         const int z = item / pl.own_tiles;
-        slot = pl.prefix_splits + z;
+        slot = pl.prefix_slots + z;
         q0 = request_start(ba, b);
         const int qn = min(request_start(ba, b + 1), total) - q0, len = own_len(p, b, lane);
         row0 = (item - z * pl.own_tiles) * RT;
@@ -551,7 +551,7 @@ __global__ void __launch_bounds__(128) k_pages_merge(PagesAttention p, PagesPlan
         int chunk;
         own_chunks(own_len(p, b, lane), pl.own_splits, chunk, n_own);
     }
-    const int n = pl.prefix_splits + n_own;
+    const int n = pl.prefix_slots + (n_own << pl.own_alt);
     const long long step = (long long)ba.T * p.nh, at = (long long)t * p.nh + h;
     float M = -INFINITY;
     for (int s = lane; s < n; s += 32) M = fmaxf(M, pl.ml[(s * step + at) * 2]);
@@ -585,26 +585,45 @@ __global__ void __launch_bounds__(128) k_pages_merge(PagesAttention p, PagesPlan
     if (p.lse && lane == 0) p.lse[at] = row_lse(M, L);
 }
 
+// Which kernel takes what. k_pages_tc pads a row tile to 128 rows and needs an SM to itself;
+// k_pages_rows reads K and V again for every 16 rows (8 with fp32 queries).
+constexpr int kSms = 148;
+constexpr int kTcMinRows = 32;
+constexpr int kTcMinOwnRows = 64;
 PagesPlan plan_attention(const PagesAttention &p) {
     PagesPlan pl{};
     const PageBatchView &ba = p.ba;
-    const int G = p.nh / p.pg.nkv, rt = p.q_type == VT_F32 ? 8 : 16;
-    const long long want = 2 * 148;                          // CTAs that fill the GPU twice
-    const long long bound = (long long)ba.table_width * p.pg.page_size;
     const auto up = [](long long a, long long b) { return (a + b - 1) / b; };
+    const bool f32 = p.q_type == VT_F32, fits = pages_tc_fits(p.pg);
+    const int G = p.nh / p.pg.nkv, rt = f32 ? 8 : 16, nkv = p.pg.nkv;
+    const long long rows = (long long)ba.T * G, own_rows = (long long)std::min(ba.max_q, ba.T) * G;
+    const long long bound = (long long)ba.table_width * p.pg.page_size;
+    const int pair = f32 ? 128 : 256;                        // rows of a k_pages_tc CTA that needs no partner
+    if (fits && bound > 0 && own_rows > 128 && rows * nkv / pair >= 96) {
+        pl.whole = pl.own_tc = 1;
+        pl.own_tiles = (int)up(own_rows, pair);
+        pl.slots = 1;
+        return pl;
+    }
+    const auto splits = [&](long long ctas, long long want, long long keys) {   // key ranges that fill the GPU
+        return std::min<long long>({std::max<long long>(1, want / ctas), up(keys, kPagesOwnKeys), kPagesMaxSplits});
+    };
     if (ba.prefix_len > 0) {
-        pl.prefix_tiles = (int)up((long long)ba.T * G, rt);
-        long long n = std::max<long long>(1, want / ((long long)pl.prefix_tiles * p.pg.nkv));
-        n = std::min<long long>({n, up(ba.prefix_len, 256), kPagesMaxSplits});
+        pl.prefix_tc = fits && rows > kTcMinRows;
+        pl.prefix_alt = pl.prefix_tc && (f32 || rows <= 128);
+        pl.prefix_tiles = (int)up(rows, !pl.prefix_tc ? rt : pl.prefix_alt ? 128 : 256);
+        const long long n = splits((long long)pl.prefix_tiles * nkv, pl.prefix_tc ? kSms : 2 * kSms, ba.prefix_len);
         pl.prefix_chunk = (int)(up(up(ba.prefix_len, n), kPagesGrain) * kPagesGrain);
         pl.prefix_splits = (int)up(ba.prefix_len, pl.prefix_chunk);
+        pl.prefix_slots = pl.prefix_splits << pl.prefix_alt;
     }
     if (bound > 0) {
-        pl.own_tiles = (int)up((long long)ba.max_q * G, rt);
-        const long long n = std::max<long long>(1, want / ((long long)ba.B * pl.own_tiles * p.pg.nkv));
-        pl.own_splits = (int)std::min<long long>({n, up(bound, 256), kPagesMaxSplits});
+        pl.own_tc = fits && own_rows > kTcMinOwnRows;
+        pl.own_alt = pl.own_tc && (f32 || own_rows <= 128);
+        pl.own_tiles = (int)up(own_rows, !pl.own_tc ? rt : pl.own_alt ? 128 : 256);
+        pl.own_splits = (int)splits((long long)ba.B * pl.own_tiles * nkv, pl.own_tc ? kSms : 2 * kSms, bound);
     }
-    pl.slots = pl.prefix_splits + pl.own_splits;
+    pl.slots = pl.prefix_slots + (pl.own_splits << pl.own_alt);
     return pl;
 }
 size_t plan_bytes(const PagesAttention &p, const PagesPlan &pl) {
@@ -615,7 +634,12 @@ template <int HD, typename TQ, typename TC>
 cudaError_t attention_typed(const PagesAttention &p, PagesPlan pl, cudaStream_t s) {
     pl.acc = static_cast<float *>(p.ws);
     pl.ml = pl.acc + (size_t)pl.slots * p.ba.T * p.nh * HD;
-    const int items = pl.prefix_tiles * pl.prefix_splits + p.ba.B * pl.own_tiles * pl.own_splits;
+    if (pl.prefix_tc || pl.own_tc) {
+        const cudaError_t e = launch_pages_tc(p, pl, s);
+        if (e != cudaSuccess || pl.whole) return e;
+    }
+    const int items = (pl.prefix_tc ? 0 : pl.prefix_tiles * pl.prefix_splits) +
+                      (pl.own_tc ? 0 : p.ba.B * pl.own_tiles * pl.own_splits);
     cudaError_t e = raise_smem(k_pages_rows<HD, TQ, TC>, kRowsSmem);
     if (e != cudaSuccess) return e;
     if (items > 0) k_pages_rows<HD, TQ, TC><<<dim3(items, p.pg.nkv), 32 * kRowsWarps, kRowsSmem, s>>>(p, pl);

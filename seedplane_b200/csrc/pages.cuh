@@ -103,8 +103,12 @@ constexpr int kPagesGrain = 128;                             // key ranges are m
 constexpr int kPagesOwnKeys = 256;                           // own keys per range at least
 constexpr int kPagesMaxSplits = 32;
 struct PagesPlan {
-    int prefix_tiles, prefix_splits, prefix_chunk;           // row tiles of the whole batch x key ranges
-    int own_tiles, own_splits;                               // row tiles of a request x key ranges at most
+    // all rows over ranges of the prefix, each request's rows over ranges of its own keys: row tiles x key
+    // ranges; `tc`: k_pages_tc (else k_pages_rows); `alt`: its two groups of warps take alternate key tiles
+    // of one row tile and leave a partial each
+    int prefix_tiles, prefix_splits, prefix_chunk, prefix_slots, prefix_tc, prefix_alt;
+    int own_tiles, own_splits, own_tc, own_alt;
+    int whole;                                               // own_tiles over the prefix and the own keys, no partials
     int slots;                                               // partials per (token, head); 1: no merge
     float *acc, *ml;                                         // [slots][T][heads][hd], [slots][T][heads][m, l]
 };
@@ -114,6 +118,10 @@ SP_DEVINL void own_chunks(int len, int most, int &chunk, int &n) {
     chunk = max(kPagesGrain, ((len + want - 1) / want + kPagesGrain - 1) / kPagesGrain * kPagesGrain);
     n = max(1, (len + chunk - 1) / chunk);                   // no key: one empty range
 }
+
+// pages_tc.cu
+bool pages_tc_fits(const PagesView &pg);
+cudaError_t launch_pages_tc(const PagesAttention &p, const PagesPlan &pl, cudaStream_t s);
 
 // Raise a kernel's dynamic shared memory limit, once per device and kernel.
 template <typename... KArgs>

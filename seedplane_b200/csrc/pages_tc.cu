@@ -1,0 +1,597 @@
+// Attention of many rows over pages on the 5th-generation tensor cores, sm_100a: the shared prefix under the
+// stacked rows of a whole batch, and requests that bring many tokens (sp_pages_attention).
+//
+// A CTA takes up to 256 (token, head) rows of one kv head's group and walks a key sequence (a range of the
+// prefix, or the prefix and then one request's own keys) in tiles of 128 keys:
+//   S_q = Q_q K^T    tcgen05.mma M 128, N 128 into TMEM (two row tiles q, 128 columns each)
+//   P_q = 2^(S c - m), m the row's running maximum, kept while it grows by less than 2^8, so that the sums
+//         and O seldom need rescaling (P <= 256 then, exact in either 16-bit type's range); written over
+//         S_q in TMEM in the cache's type
+//   O_q += P_q V     tcgen05.mma with A = P_q in TMEM, B = V as it lies in its pages (MN-major)
+// Bound by the exponentials (16 a clock and SM) and the MMAs, which take equally long for head_dim 128:
+//   warps 0-3, 4-7   one row tile each: thread = row. tcgen05.ld of 128 scores, maximum, exponentials, tcgen05.st
+//   warp 8           TMA of the pages' rows (64 dims x a page's slots a box, 128-byte swizzle) into a ring
+//   warp 9           issues the MMAs: while one row tile's scores are exponentiated, the other's products run
+// One row tile alone (at most 128 rows: a small batch, or fp32 queries) gives both groups of warps work by
+// taking alternate key tiles, each with its own (m, l, O); their partials are joined like those of key ranges.
+// fp32 queries: Q as fp16 hi and lo tiles, S = Qhi K^T + Qlo K^T, P as hi and lo, O += Phi V + Plo V.
+// Slots of a page behind the last key may hold anything: their scores are replaced, their V rows zeroed in
+// shared memory (0 x NaN would reach O). Every wait is bounded.
+#include <cuda.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "pages.cuh"
+#include "tc.cuh"
+
+namespace sp {
+
+namespace {
+
+constexpr int kTcKeys = 128;                 // keys of a tile
+constexpr int kTcRows = 128;                 // rows of a row tile
+constexpr int kTcThreads = 384;              // warps 10, 11 only fill the third warpgroup
+constexpr int kTcProducer = 8, kTcMma = 9;   // warps
+constexpr int kTcStages = 4;
+constexpr uint32_t kTcSpin = 1u << 22;
+constexpr float kTcGrow = 8.0f;              // log2 of the growth a running maximum may lag behind
+
+template <int HD>
+struct TcSmem {
+    static constexpr int kHalf = kTcKeys * 128;              // 64 dims of 128 rows
+    static constexpr int kTile = kHalf * (HD / 64);          // a K, V or Q tile
+    static constexpr int kQ = 2 * kTile;                     // two row tiles, or hi and lo
+    static constexpr int kBytes = kQ + kTcStages * kTile + 1024;
+};
+
+SP_DEVINL void tma_page(uint32_t dst, const CUtensorMap *map, int d, int slot, int head, int page, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(d), "r"(slot), "r"(head), "r"(page), "r"(smem_u32(bar))
+        : "memory");
+}
+// V rows as the B operand: dims contiguous (MN-major), 64 dims a 128-byte row, 8 keys a swizzle atom; the
+// next 64 dims lie kHalf bytes on, the next 8 keys 1,024.
+SP_DEVINL uint64_t v_desc(uint32_t addr, uint32_t half) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(half >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) |
+           (2ull << 61);
+}
+// A from TMEM (16-bit values, two a column)
+SP_DEVINL void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate));
+}
+SP_DEVINL void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]));
+}
+SP_DEVINL void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+          "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+          "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]));
+}
+SP_DEVINL void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Instruction descriptor: D fp32, A and B of the cache's type, M 128, N = n; B MN-major or K-major.
+template <typename TC>
+SP_DEVINL constexpr uint32_t tc_idesc(int n, bool mn) {
+    const uint32_t fmt = std::is_same<TC, __half>::value ? 0u : 1u;
+    return (1u << 4) | (fmt << 7) | (fmt << 10) | ((mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+struct TcBarriers {
+    uint64_t full[kTcStages], empty[kTcStages];
+    uint64_t q_full, s_full[2], p_full[2], o_full[2], tail, drain;
+};
+
+// The keys an item walks: tiles [0, n_a) of the first segment, then [n_a, n) of the second.
+struct TcKeys {
+    const int *table_a, *table_b;
+    int lo_a, hi_a, hi_b;                    // first segment [lo_a, hi_a), second [0, hi_b)
+    int n_a, n;
+    SP_DEVINL int lo(int i) const { return i < n_a ? lo_a + i * kTcKeys : (i - n_a) * kTcKeys; }
+    SP_DEVINL int hi(int i) const { return i < n_a ? hi_a : hi_b; }
+    SP_DEVINL const int *table(int i) const { return i < n_a ? table_a : table_b; }
+};
+
+struct TcWait {
+    volatile int *abort;
+    int *status;
+    SP_DEVINL bool wait(uint64_t *bar, uint32_t parity) const {
+        for (uint32_t i = 0; i < kTcSpin; ++i) {
+            if (mbar_try_wait(bar, parity)) return true;
+            if ((i & 127u) == 127u && *abort) return false;
+        }
+        *abort = 1;
+        if (status) atomicCAS(status, 0, kErrMbarTimeout);
+        return false;
+    }
+    // by a whole warp: the same answer in every lane
+    SP_DEVINL bool wait_warp(uint64_t *bar, uint32_t parity) const { return __all_sync(0xffffffffu, wait(bar, parity)); }
+};
+
+template <int HD, typename TQ, typename TC>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    k_pages_tc(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, PagesAttention p,
+               PagesPlan pl) {
+    constexpr bool kSplit = sizeof(TQ) == 4;
+    using L = TcSmem<HD>;
+    constexpr int CH = HD / 8, KS = HD / 16;
+    extern __shared__ uint8_t tc_smem_raw[];
+    __shared__ __align__(8) TcBarriers bar;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const PageBatchView &ba = p.ba;
+    const int g = blockIdx.y, G = p.nh / p.pg.nkv;
+    // the item
+    const int total = total_rows(ba);
+    int q0 = 0, row0, nrows, slot = 0, own0 = INT_MAX / 2, own_tile0 = INT_MAX, item = blockIdx.x;
+    bool alt = false;                        // the groups of warps take alternate key tiles of one row tile
+    TcKeys ks{};
+    const int n_prefix = pl.prefix_tc ? pl.prefix_tiles * pl.prefix_splits : 0;
+    if (item < n_prefix) {                   // all rows over a range of the prefix
+        alt = pl.prefix_alt;
+        const int z = item / pl.prefix_tiles, tile_rows = alt ? kTcRows : 2 * kTcRows;
+        row0 = (item - z * pl.prefix_tiles) * tile_rows;
+        nrows = min(tile_rows, total * G - row0);
+        slot = z << pl.prefix_alt;
+        ks.table_a = ba.prefix;
+        ks.lo_a = z * pl.prefix_chunk;
+        ks.hi_a = min(ba.prefix_len, ks.lo_a + pl.prefix_chunk);
+        ks.n = ks.n_a = (ks.hi_a - ks.lo_a + kTcKeys - 1) / kTcKeys;
+        if (nrows <= 0) return;
+    } else {                                 // a request's rows over its own keys, or the prefix and them
+        alt = pl.own_alt;
+        item -= n_prefix;
+        const int per = pl.own_tiles * (pl.whole ? 1 : pl.own_splits), b = item / per;
+        item -= b * per;
+        const int z = item / pl.own_tiles, tile_rows = alt || kSplit ? kTcRows : 2 * kTcRows;
+        row0 = (pl.own_tiles - 1 - (item - z * pl.own_tiles)) * tile_rows;    // the longest first
+        q0 = request_start(ba, b);
+        const int qn = min(request_start(ba, b + 1), total) - q0, len = own_len(p, b, tid);
+        if (qn > ba.max_q && tid == 0) set_status(p.pg.status);
+        nrows = min(tile_rows, qn * G - row0);
+        if (nrows <= 0) return;
+        own0 = len - qn;
+        const int last = max(0, min(len, own0 + (row0 + nrows - 1) / G + 1));
+        const int *table = ba.tables + (long long)b * ba.table_stride;
+        if (pl.whole) {
+            ks.table_a = ba.prefix;
+            ks.hi_a = ba.prefix_len;
+            ks.table_b = table;
+            ks.hi_b = last;
+            ks.n_a = (ks.hi_a + kTcKeys - 1) / kTcKeys;
+            ks.n = ks.n_a + (last + kTcKeys - 1) / kTcKeys;
+            own_tile0 = ks.n_a;
+        } else {
+            int chunk, parts;
+            own_chunks(len, pl.own_splits, chunk, parts);
+            if (z >= parts) return;
+            slot = pl.prefix_slots + (z << pl.own_alt);
+            ks.table_a = table;
+            ks.lo_a = z * chunk;
+            ks.hi_a = min(ks.lo_a + chunk, last);
+            ks.n = ks.n_a = max(0, (ks.hi_a - ks.lo_a + kTcKeys - 1) / kTcKeys);
+            own_tile0 = 0;
+        }
+    }
+    const int n = ks.n;
+    const int nq = alt || nrows > kTcRows ? 2 : 1;           // groups of softmax warps at work
+    const uint32_t base = (smem_u32(tc_smem_raw) + 1023u) & ~1023u, ring = base + L::kQ;
+    const TcWait w{&s_abort, p.pg.status};
+
+    if (tid == 0) {
+        s_abort = 0;
+        for (int i = 0; i < kTcStages; ++i) {
+            mbar_init(&bar.full[i], 1);
+            mbar_init(&bar.empty[i], 1);
+        }
+        mbar_init(&bar.q_full, 256);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bar.s_full[i], 1);
+            mbar_init(&bar.p_full[i], 128);
+            mbar_init(&bar.o_full[i], 1);
+        }
+        mbar_init(&bar.tail, 1);
+        mbar_init(&bar.drain, 1);
+        fence_mbar_init();
+    }
+    if (warp == kTcMma) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512u));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+
+    // 384 threads of 168 registers at launch: the softmax groups take 224, the third 56 (the sum is the same)
+    if (warp >= kTcProducer) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == kTcProducer) {
+        // ring order: K of the first `lead` tiles, then V of tile i and K of tile i + lead
+        const int lead = alt ? 2 : 1;
+        int it = 0, tails = 0;
+        const auto load = [&](int i, bool is_v) -> bool {
+            const int st = it % kTcStages;
+            if (it >= kTcStages && !w.wait_warp(&bar.empty[st], (uint32_t)(it / kTcStages - 1) & 1u)) return false;
+            const int lo = ks.lo(i), keys = min(kTcKeys, ks.hi(i) - lo);
+            const int per = min(p.pg.page_size, kTcKeys), pages = (keys + per - 1) / per;
+            const uint32_t dst = ring + (uint32_t)st * L::kTile;
+            const bool tail = is_v && keys < kTcKeys;
+            uint64_t *b = tail ? &bar.tail : &bar.full[st];
+            int page = 0, slot0 = 0;
+            if (lane < pages) {
+                const int key = lo + lane * per;
+                const int pi = key / p.pg.page_size;
+                page = ks.table(i)[pi];
+                slot0 = key - pi * p.pg.page_size;
+                if ((unsigned)page >= (unsigned)p.pg.n_pages) {
+                    set_status(p.pg.status);
+                    page = p.pg.n_pages;     // outside the tensor: zeros
+                }
+            }
+            if (lane == 0) mbar_arrive_expect_tx(b, (uint32_t)(pages * per) * HD * 2);
+            __syncwarp();
+            if (lane < pages) {
+#pragma unroll
+                for (int h = 0; h < HD / 64; ++h)
+                    tma_page(dst + h * L::kHalf + lane * per * 128, is_v ? &tm_v : &tm_k, 64 * h, slot0, g, page, b);
+            }
+            __syncwarp();
+            if (tail) {                      // rows behind the last key: zero, once the page's slots are there
+                if (!w.wait_warp(&bar.tail, (uint32_t)tails++ & 1u)) return false;
+                for (int r = keys * CH + lane; r < kTcKeys * CH; r += 32) {
+                    const int row = r / CH, c = r - row * CH;
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(dst + (c >> 3) * L::kHalf + row * 128 + (c & 7) * 16), "r"(0u)
+                                 : "memory");
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar.full[st]);
+            }
+            ++it;
+            return true;
+        };
+        int kc = 0, vc = 0;
+        for (bool ok = true; ok && vc < n;) {
+            const bool is_v = kc >= n || kc >= vc + lead;
+            ok = load(is_v ? vc : kc, is_v);
+            ++(is_v ? vc : kc);
+        }
+        // no copy is in flight when the CTA ends, whoever gave up
+        for (int j = max(0, it - kTcStages); j < it; ++j)
+            for (uint32_t k = 0; k < kTcSpin && !mbar_try_wait(&bar.full[j % kTcStages], (uint32_t)(j / kTcStages) & 1u); ++k) {
+            }
+        } else if (warp == kTcMma) {
+        if (lane == 0 && n > 0 && w.wait(&bar.q_full, 0)) {
+            constexpr uint32_t id_s = tc_idesc<TC>(kTcKeys, false), id_o = tc_idesc<TC>(HD, true);
+            int it = 0;
+            bool ok = true;
+            int k_st = 0, v_st = 0;
+            uint32_t p_ph[2] = {0u, 0u};
+            const auto arrive = [&](int &st) {               // the ring's next tile
+                st = it % kTcStages;
+                ok = w.wait(&bar.full[st], (uint32_t)(it / kTcStages) & 1u);
+                ++it;
+                tc_fence_after();
+                return ok;
+            };
+            const auto scores = [&](int q) {                 // S_q = Q K^T
+                const uint32_t kt = ring + (uint32_t)k_st * L::kTile;
+#pragma unroll 1
+                for (int part = 0; part < (kSplit ? 2 : 1); ++part) {
+                    const uint32_t qt = base + (uint32_t)(kSplit ? part : alt ? 0 : q) * L::kTile;
+#pragma unroll 1
+                    for (int kk = 0; kk < KS; ++kk) {
+                        const uint32_t o = (uint32_t)(kk >> 2) * L::kHalf + (uint32_t)(kk & 3) * 32;
+                        mma_f16_id(tmem + 128 * q, smem_desc_sw128(qt + o, 1024), smem_desc_sw128(kt + o, 1024), id_s,
+                                   part + kk > 0);
+                    }
+                }
+                mma_commit(&bar.s_full[q]);
+            };
+            const auto values = [&](int q, bool first) -> bool {                      // O_q += P_q V
+                if (!w.wait(&bar.p_full[q], p_ph[q])) return ok = false;
+                p_ph[q] ^= 1u;
+                tc_fence_after();
+                const uint32_t vt = ring + (uint32_t)v_st * L::kTile;
+#pragma unroll 1
+                for (int part = 0; part < (kSplit ? 2 : 1); ++part)
+#pragma unroll 1
+                    for (int kk = 0; kk < kTcKeys / 16; ++kk)
+                        mma_ts(tmem + 256 + 128 * q, tmem + 128 * q + 64 * part + 8 * kk, v_desc(vt + kk * 2048, L::kHalf), id_o,
+                               !(first && part + kk == 0));
+                return true;
+            };
+            if (alt) {
+                for (int i = 0; i < 2 && i < n && ok; ++i) {
+                    if (!arrive(k_st)) break;
+                    scores(i);
+                    mma_commit(&bar.empty[k_st]);
+                }
+                for (int i = 0; i < n && ok; ++i) {
+                    if (!arrive(v_st) || !values(i & 1, i < 2)) break;
+                    mma_commit(&bar.empty[v_st]);
+                    if (i + 2 < n) {
+                        if (!arrive(k_st)) break;
+                        scores(i & 1);
+                        mma_commit(&bar.empty[k_st]);
+                    } else {
+                        mma_commit(&bar.o_full[i & 1]);
+                    }
+                }
+            } else {
+                if (arrive(k_st)) {
+                    for (int q = 0; q < nq; ++q) scores(q);
+                    mma_commit(&bar.empty[k_st]);
+                }
+                for (int i = 0; i < n && ok; ++i) {
+                    for (int q = 0; q < nq && ok; ++q) {
+                        if (q == 0 && !arrive(v_st)) break;
+                        if (!values(q, i == 0)) break;
+                        if (q == nq - 1) mma_commit(&bar.empty[v_st]);
+                        if (i + 1 < n) {
+                            if (q == 0 && !arrive(k_st)) break;
+                            scores(q);
+                            if (q == nq - 1) mma_commit(&bar.empty[k_st]);
+                        } else {
+                            mma_commit(&bar.o_full[q]);
+                        }
+                    }
+                }
+            }
+            if (!ok) {                       // gave up: the MMAs in flight read this CTA's memory
+                mma_commit(&bar.drain);
+                for (uint32_t k = 0; k < kTcSpin && !mbar_try_wait(&bar.drain, 0); ++k) {
+                }
+            }
+        }
+        __syncwarp();
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int grp = warp >> 2;
+        const TQ *qbase = reinterpret_cast<const TQ *>(p.q);
+        // Q rows into swizzled tiles (rows behind the last: zero)
+        const int fill = (alt || nq == 1 ? 1 : 2) * kTcRows;
+        for (int i = tid; i < fill * CH; i += 256) {
+            const int r = i / CH, c = i - r * CH;
+            const uint32_t at = base + (uint32_t)(r >> 7) * L::kTile + (c >> 3) * L::kHalf + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4);
+            const int row = row0 + r;
+            const TQ *src = qbase + (long long)(q0 + row / G) * p.q_stride + (g * G + row % G) * HD + c * 8;
+            uint4 v = make_uint4(0u, 0u, 0u, 0u), lo = v;
+            if (r < nrows) {
+                if constexpr (kSplit) {
+                    const float4 a = *reinterpret_cast<const float4 *>(src), b = *(reinterpret_cast<const float4 *>(src) + 1);
+                    const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                    uint32_t hw[4], lw[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        float h0, h1;
+                        hw[k] = pack2<TC>(x[2 * k], x[2 * k + 1]);
+                        unpack2<TC>(hw[k], h0, h1);
+                        lw[k] = pack2<TC>(x[2 * k] - h0, x[2 * k + 1] - h1);
+                    }
+                    v = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+                    lo = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+                } else {
+                    v = *reinterpret_cast<const uint4 *>(src);
+                }
+            }
+            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+            if constexpr (kSplit)
+                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at + L::kTile), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w)
+                             : "memory");
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&bar.q_full);
+        if (grp < nq) {
+            const int r = (alt ? 0 : grp * kTcRows) + (warp & 3) * 32 + lane, row = row0 + r;
+            const bool live = r < nrows;
+            const int seen = live ? own0 + row / G + 1 : 0;  // own keys this row sees: below this
+            const uint32_t lanes = (uint32_t)(warp & 3) * 32u << 16;
+            const uint32_t ts = tmem + lanes + 128u * grp, to = tmem + lanes + 256u + 128u * grp;
+            const float c = p.scale * 1.4426950408889634f;
+            float m = -INFINITY, l = 0.f;
+            uint32_t ph = 0u;
+            bool ok = true, any = false;
+            for (int i = alt ? grp : 0; i < n; i += alt ? 2 : 1) {
+                if (!w.wait_warp(&bar.s_full[grp], ph)) { ok = false; break; }
+                ph ^= 1u;
+                tc_fence_after();
+                uint32_t s[4][32];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) tmem_ld32_nowait(ts + 32 * k, s[k]);
+                tmem_wait_ld();
+                const int lo = ks.lo(i), lim = min(ks.hi(i), i >= own_tile0 ? seen : INT_MAX) - lo;
+                if (__any_sync(0xffffffffu, lim < kTcKeys)) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (32 * k + j >= lim) s[k][j] = 0xff800000u;             // -inf
+                }
+                float mx[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    mx[k] = __uint_as_float(s[k][0]);
+#pragma unroll
+                    for (int j = 1; j < 32; ++j) mx[k] = fmaxf(mx[k], __uint_as_float(s[k][j]));
+                }
+                const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+                const bool grow = mt > m + kTcGrow || (!any && mt > m);
+                if (any) {
+                    // sfull of this tile came after the products of the tile before: O is at rest
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float f = grow ? exp2_approx(m - mt) : 1.f;
+                        l *= f;
+#pragma unroll
+                        for (int k = 0; k < HD / 32; ++k) {
+                            uint32_t o[32];
+                            tmem_ld32_nowait(to + 32 * k, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                            tmem_st32(to + 32 * k, o);
+                        }
+                    }
+                }
+                if (grow) m = mt;
+                any = true;
+                const float ms = m == -INFINITY ? 0.f : m;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    uint32_t hi[16], lw[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const float e0 = exp2_approx(fmaf(__uint_as_float(s[k][2 * j]), c, -ms));
+                        const float e1 = exp2_approx(fmaf(__uint_as_float(s[k][2 * j + 1]), c, -ms));
+                        sum[j & 3] += e0 + e1;
+                        hi[j] = pack2<TC>(e0, e1);
+                        if constexpr (kSplit) {
+                            float h0, h1;
+                            unpack2<TC>(hi[j], h0, h1);
+                            lw[j] = pack2<TC>(e0 - h0, e1 - h1);
+                        }
+                    }
+                    tmem_st16(ts + 16 * k, hi);
+                    if constexpr (kSplit) tmem_st16(ts + 64 + 16 * k, lw);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(&bar.p_full[grp]);
+            }
+            // O and the row's statistics
+            if (any && ok) ok = w.wait_warp(&bar.o_full[grp], 0);
+            tc_fence_after();
+            const long long rt = q0 + row / G, hh = g * G + row % G;
+            const long long at = ((long long)(slot + (alt ? grp : 0)) * ba.T + rt) * p.nh + hh;
+            const bool direct = pl.slots == 1;
+            const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+            for (int k = 0; k < HD / 32; ++k) {
+                uint32_t o[32];
+                if (any && ok) {
+                    tmem_ld32_nowait(to + 32 * k, o);
+                    tmem_wait_ld();
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) o[j] = 0u;
+                }
+                if (live && direct) {
+                    TQ *dst = reinterpret_cast<TQ *>(p.out) + rt * p.out_stride + hh * HD + 32 * k;
+                    float v[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = l == l ? __uint_as_float(o[j]) * inv : l;
+                    if constexpr (kSplit) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            reinterpret_cast<float4 *>(dst)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            reinterpret_cast<uint4 *>(dst)[j] =
+                                make_uint4(pack2<TQ>(v[8 * j], v[8 * j + 1]), pack2<TQ>(v[8 * j + 2], v[8 * j + 3]),
+                                           pack2<TQ>(v[8 * j + 4], v[8 * j + 5]), pack2<TQ>(v[8 * j + 6], v[8 * j + 7]));
+                    }
+                } else if (live) {
+                    uint4 *dst = reinterpret_cast<uint4 *>(pl.acc + at * HD + 32 * k);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) dst[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                }
+                __syncwarp();
+            }
+            if (live) {
+                if (direct) {
+                    if (p.lse) p.lse[rt * p.nh + hh] = row_lse(m, l);
+                } else {
+                    *reinterpret_cast<float2 *>(pl.ml + at * 2) = make_float2(m, l);
+                }
+            }
+            tc_fence_before();
+        }
+    }
+    __syncthreads();
+    if (warp == kTcMma) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+    }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_tiled() {
+    static const EncodeTiledFn fn = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &r) != cudaSuccess ||
+            r != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<EncodeTiledFn>(f);
+    }();
+    return fn;
+}
+
+// [dims][slots][heads][pages] of one of K and V; a box is 64 dims of a page's slots (128 at most)
+cudaError_t pages_map(CUtensorMap *m, const PagesView &pg, void *base, bool bf16) {
+    const EncodeTiledFn enc = encode_tiled();
+    if (!enc) return cudaErrorNotSupported;
+    const cuuint64_t dims[4] = {(cuuint64_t)pg.hd, (cuuint64_t)pg.page_size, (cuuint64_t)pg.nkv, (cuuint64_t)pg.n_pages};
+    // a dimension of one entry has no stride of its own
+    const cuuint64_t any = (cuuint64_t)pg.hd * 2;
+    const cuuint64_t strides[3] = {pg.page_size > 1 ? (cuuint64_t)pg.slot_stride * 2 : any,
+                                   pg.nkv > 1 ? (cuuint64_t)pg.head_stride * 2 : any,
+                                   pg.n_pages > 1 ? (cuuint64_t)pg.page_stride * 2 : any};
+    const cuuint32_t box[4] = {64, (cuuint32_t)std::min(pg.page_size, kTcKeys), 1, 1}, one[4] = {1, 1, 1, 1};
+    const CUresult r = enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base, dims, strides, box,
+                           one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+template <int HD, typename TQ, typename TC>
+cudaError_t tc_typed(const PagesAttention &p, const PagesPlan &pl, cudaStream_t s) {
+    CUtensorMap k, v;
+    cudaError_t e = pages_map(&k, p.pg, p.pg.k, !std::is_same<TC, __half>::value);
+    if (e == cudaSuccess) e = pages_map(&v, p.pg, p.pg.v, !std::is_same<TC, __half>::value);
+    if (e == cudaSuccess) e = raise_smem(k_pages_tc<HD, TQ, TC>, TcSmem<HD>::kBytes);
+    if (e != cudaSuccess) return e;
+    const int items = (pl.prefix_tc ? pl.prefix_tiles * pl.prefix_splits : 0) +
+                      (pl.own_tc ? p.ba.B * pl.own_tiles * (pl.whole ? 1 : pl.own_splits) : 0);
+    k_pages_tc<HD, TQ, TC><<<dim3(items, p.pg.nkv), kTcThreads, TcSmem<HD>::kBytes, s>>>(k, v, p, pl);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+// Pages whose slots a TMA box takes whole and whose rows land on swizzle atoms.
+bool pages_tc_fits(const PagesView &pg) {
+    const bool pow2 = pg.page_size >= 8 && pg.page_size <= 4096 && (pg.page_size & (pg.page_size - 1)) == 0;
+    const auto ok = [](long long s) { return s > 0 && s < (1ll << 38); };
+    return pow2 && ok(pg.slot_stride) && (pg.nkv == 1 || ok(pg.head_stride)) && (pg.n_pages == 1 || ok(pg.page_stride)) &&
+           encode_tiled() != nullptr;
+}
+
+cudaError_t launch_pages_tc(const PagesAttention &p, const PagesPlan &pl, cudaStream_t s) {
+    const bool wide = p.pg.hd == 128;
+    if (p.q_type == VT_F32)
+        return wide ? tc_typed<128, float, __half>(p, pl, s) : tc_typed<64, float, __half>(p, pl, s);
+    if (p.q_type == VT_F16)
+        return wide ? tc_typed<128, __half, __half>(p, pl, s) : tc_typed<64, __half, __half>(p, pl, s);
+    return wide ? tc_typed<128, __nv_bfloat16, __nv_bfloat16>(p, pl, s) : tc_typed<64, __nv_bfloat16, __nv_bfloat16>(p, pl, s);
+}
+
+}  // namespace sp
