@@ -78,6 +78,30 @@ SP_DEVINL void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
           "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
           "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]));
 }
+// Two fp32 values as one 64-bit operand of the packed instructions.
+SP_DEVINL uint64_t f2(float a, float b) { return (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32); }
+SP_DEVINL float f2_lo(uint64_t v) { return __uint_as_float((uint32_t)v); }
+SP_DEVINL float f2_hi(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+SP_DEVINL uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+SP_DEVINL uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+SP_DEVINL float max3(float a, float b, float c) {             // NaN is passed over, as by fmaxf
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+SP_DEVINL bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
 SP_DEVINL void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Instruction descriptor: D fp32, A and B of the cache's type, M 128, N = n; B MN-major or K-major.
@@ -273,7 +297,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             for (uint32_t k = 0; k < kTcSpin && !mbar_try_wait(&bar.full[j % kTcStages], (uint32_t)(j / kTcStages) & 1u); ++k) {
             }
         } else if (warp == kTcMma) {
-        if (lane == 0 && n > 0 && w.wait(&bar.q_full, 0)) {
+        // the whole warp runs the loop, one elected lane issues: control flow and descriptors stay uniform
+        if (n > 0 && w.wait_warp(&bar.q_full, 0)) {
             constexpr uint32_t id_s = tc_idesc<TC>(kTcKeys, false), id_o = tc_idesc<TC>(HD, true);
             int it = 0;
             bool ok = true;
@@ -281,77 +306,84 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             uint32_t p_ph[2] = {0u, 0u};
             const auto arrive = [&](int &st) {               // the ring's next tile
                 st = it % kTcStages;
-                ok = w.wait(&bar.full[st], (uint32_t)(it / kTcStages) & 1u);
+                ok = w.wait_warp(&bar.full[st], (uint32_t)(it / kTcStages) & 1u);
                 ++it;
                 tc_fence_after();
                 return ok;
             };
+            const auto commit = [&](uint64_t *b) {
+                if (elect_one()) mma_commit(b);
+                __syncwarp();
+            };
             const auto scores = [&](int q) {                 // S_q = Q K^T
-                const uint32_t kt = ring + (uint32_t)k_st * L::kTile;
-#pragma unroll 1
-                for (int part = 0; part < (kSplit ? 2 : 1); ++part) {
-                    const uint32_t qt = base + (uint32_t)(kSplit ? part : alt ? 0 : q) * L::kTile;
-#pragma unroll 1
-                    for (int kk = 0; kk < KS; ++kk) {
-                        const uint32_t o = (uint32_t)(kk >> 2) * L::kHalf + (uint32_t)(kk & 3) * 32;
-                        mma_f16_id(tmem + 128 * q, smem_desc_sw128(qt + o, 1024), smem_desc_sw128(kt + o, 1024), id_s,
-                                   part + kk > 0);
-                    }
+                const uint64_t kd = smem_desc_sw128(ring + (uint32_t)k_st * L::kTile, 1024);
+                const uint64_t qd = smem_desc_sw128(base + (uint32_t)(kSplit || alt ? 0 : q) * L::kTile, 1024);
+                if (elect_one()) {
+#pragma unroll
+                    for (int part = 0; part < (kSplit ? 2 : 1); ++part)
+#pragma unroll
+                        for (int kk = 0; kk < KS; ++kk) {
+                            const int o = ((kk >> 2) * L::kHalf + (kk & 3) * 32) >> 4;
+                            mma_f16_id(tmem + 128 * q, qd + o + ((part * L::kTile) >> 4), kd + o, id_s, part + kk > 0);
+                        }
+                    mma_commit(&bar.s_full[q]);
                 }
-                mma_commit(&bar.s_full[q]);
+                __syncwarp();
             };
             const auto values = [&](int q, bool first) -> bool {                      // O_q += P_q V
-                if (!w.wait(&bar.p_full[q], p_ph[q])) return ok = false;
+                const uint64_t vd = v_desc(ring + (uint32_t)v_st * L::kTile, L::kHalf);
+                if (!w.wait_warp(&bar.p_full[q], p_ph[q])) return ok = false;
                 p_ph[q] ^= 1u;
                 tc_fence_after();
-                const uint32_t vt = ring + (uint32_t)v_st * L::kTile;
-#pragma unroll 1
-                for (int part = 0; part < (kSplit ? 2 : 1); ++part)
-#pragma unroll 1
-                    for (int kk = 0; kk < kTcKeys / 16; ++kk)
-                        mma_ts(tmem + 256 + 128 * q, tmem + 128 * q + 64 * part + 8 * kk, v_desc(vt + kk * 2048, L::kHalf), id_o,
-                               !(first && part + kk == 0));
+                if (elect_one()) {
+#pragma unroll
+                    for (int part = 0; part < (kSplit ? 2 : 1); ++part)
+#pragma unroll
+                        for (int kk = 0; kk < kTcKeys / 16; ++kk)
+                            mma_ts(tmem + 256 + 128 * q, tmem + 128 * q + 64 * part + 8 * kk, vd + ((kk * 2048) >> 4), id_o,
+                                   !(first && part + kk == 0));
+                }
+                __syncwarp();
                 return true;
             };
             if (alt) {
                 for (int i = 0; i < 2 && i < n && ok; ++i) {
                     if (!arrive(k_st)) break;
                     scores(i);
-                    mma_commit(&bar.empty[k_st]);
+                    commit(&bar.empty[k_st]);
                 }
                 for (int i = 0; i < n && ok; ++i) {
-                    if (!arrive(v_st) || !values(i & 1, i < 2)) break;
-                    mma_commit(&bar.empty[v_st]);
+                    // the tiles are waited for before the probabilities: only those are on the chain of waits
+                    if (!arrive(v_st) || (i + 2 < n && !arrive(k_st)) || !values(i & 1, i < 2)) break;
+                    commit(&bar.empty[v_st]);
                     if (i + 2 < n) {
-                        if (!arrive(k_st)) break;
                         scores(i & 1);
-                        mma_commit(&bar.empty[k_st]);
+                        commit(&bar.empty[k_st]);
                     } else {
-                        mma_commit(&bar.o_full[i & 1]);
+                        commit(&bar.o_full[i & 1]);
                     }
                 }
             } else {
                 if (arrive(k_st)) {
                     for (int q = 0; q < nq; ++q) scores(q);
-                    mma_commit(&bar.empty[k_st]);
+                    commit(&bar.empty[k_st]);
                 }
                 for (int i = 0; i < n && ok; ++i) {
                     for (int q = 0; q < nq && ok; ++q) {
-                        if (q == 0 && !arrive(v_st)) break;
+                        if (q == 0 && (!arrive(v_st) || (i + 1 < n && !arrive(k_st)))) break;
                         if (!values(q, i == 0)) break;
-                        if (q == nq - 1) mma_commit(&bar.empty[v_st]);
+                        if (q == nq - 1) commit(&bar.empty[v_st]);
                         if (i + 1 < n) {
-                            if (q == 0 && !arrive(k_st)) break;
                             scores(q);
-                            if (q == nq - 1) mma_commit(&bar.empty[k_st]);
+                            if (q == nq - 1) commit(&bar.empty[k_st]);
                         } else {
-                            mma_commit(&bar.o_full[q]);
+                            commit(&bar.o_full[q]);
                         }
                     }
                 }
             }
             if (!ok) {                       // gave up: the MMAs in flight read this CTA's memory
-                mma_commit(&bar.drain);
+                commit(&bar.drain);
                 for (uint32_t k = 0; k < kTcSpin && !mbar_try_wait(&bar.drain, 0); ++k) {
                 }
             }
@@ -424,9 +456,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 float mx[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    mx[k] = __uint_as_float(s[k][0]);
+                    mx[k] = fmaxf(__uint_as_float(s[k][0]), __uint_as_float(s[k][1]));
 #pragma unroll
-                    for (int j = 1; j < 32; ++j) mx[k] = fmaxf(mx[k], __uint_as_float(s[k][j]));
+                    for (int j = 2; j < 32; j += 2) mx[k] = max3(mx[k], __uint_as_float(s[k][j]), __uint_as_float(s[k][j + 1]));
                 }
                 const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
                 const bool grow = mt > m + kTcGrow || (!any && mt > m);
@@ -449,15 +481,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (grow) m = mt;
                 any = true;
                 const float ms = m == -INFINITY ? 0.f : m;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                const uint64_t c2 = f2(c, c), m2 = f2(-ms, -ms);
+                uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     uint32_t hi[16], lw[16];
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
-                        const float e0 = exp2_approx(fmaf(__uint_as_float(s[k][2 * j]), c, -ms));
-                        const float e1 = exp2_approx(fmaf(__uint_as_float(s[k][2 * j + 1]), c, -ms));
-                        sum[j & 3] += e0 + e1;
+                        const uint64_t x = fma2((uint64_t)s[k][2 * j] | ((uint64_t)s[k][2 * j + 1] << 32), c2, m2);
+                        const float e0 = exp2_approx(f2_lo(x)), e1 = exp2_approx(f2_hi(x));
+                        sum[j & 1] = add2(sum[j & 1], f2(e0, e1));
                         hi[j] = pack2<TC>(e0, e1);
                         if constexpr (kSplit) {
                             float h0, h1;
@@ -468,7 +501,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     tmem_st16(ts + 16 * k, hi);
                     if constexpr (kSplit) tmem_st16(ts + 64 + 16 * k, lw);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                sum[0] = add2(sum[0], sum[1]);
+                l += f2_lo(sum[0]) + f2_hi(sum[0]);
                 tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive(&bar.p_full[grp]);
