@@ -285,6 +285,15 @@ __global__ void __launch_bounds__(32 * kRowsWarps) k_pages_rows(PagesAttention p
     const PageBatchView &ba = p.ba;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
     const int g = blockIdx.y, G = p.nh / p.pg.nkv;
+    griddep_launch_dependents();
+    if (pl.prefix_tc || pl.own_tc) {
+        // beside k_pages_tc: the last CTA ends after that grid, so that the join, which waits for this one, waits
+        // for both
+        if (blockIdx.x == gridDim.x - 1) {
+            if (blockIdx.y == 0) griddep_wait();
+            return;
+        }
+    }
     // the item: its rows, its key range and its pages
     const int n_prefix = pl.prefix_tc ? 0 : pl.prefix_tiles * pl.prefix_splits;
     const int total = total_rows(ba);
@@ -316,7 +325,15 @@ __global__ void __launch_bounds__(32 * kRowsWarps) k_pages_rows(PagesAttention p
         if (qn > ba.max_q && threadIdx.x == 0) set_status(p.pg.status);
         int chunk, n;
         own_chunks(len, pl.own_splits, chunk, n);
-        if (nrows <= 0 || z >= n) return;
+        if (nrows <= 0) return;
+        if (z >= n) {                                        // no such range: nothing to join
+            if (threadIdx.x < nrows) {
+                const int row = row0 + threadIdx.x;
+                const long long at = ((long long)slot * ba.T + q0 + row / G) * p.nh + g * G + row % G;
+                *reinterpret_cast<float2 *>(pl.ml + at * 2) = make_float2(-INFINITY, 0.f);
+            }
+            return;
+        }
         k_max = len;
         k_lo = z * chunk;
         k_hi = min(min(len, k_lo + chunk), own0 + (row0 + nrows - 1) / G + 1);
@@ -326,33 +343,62 @@ __global__ void __launch_bounds__(32 * kRowsWarps) k_pages_rows(PagesAttention p
     const TC *kb = reinterpret_cast<const TC *>(p.pg.k) + g * p.pg.head_stride;
     const TC *vb = reinterpret_cast<const TC *>(p.pg.v) + g * p.pg.head_stride;
     const uint32_t ring = smem_u32(smem) + warp * (kRowsStages * 2 * kRowsTileBytes);
-    // a lane's key row of a tile (lane < KT): its element offset, -1 past the range or on a bad page
-    const auto row_of = [&](int tile) -> long long {
-        const int key = k_lo + tile * KT + lane;
-        if (tile >= ntiles || lane >= KT || key >= k_hi) return -1;
-        return page_row(p.pg, table, key);
+    // The page numbers of 32 pages of the walk, a lane each, so that no tile waits for its own. Pages of whole
+    // tiles (the usual case): a tile's rows are slot_stride apart; else every row looks its page up.
+    const int ps = p.pg.page_size;
+    const bool whole_tiles = ps % KT == 0;
+    int win_first = k_lo / ps, win = 0;
+    const auto fill_window = [&](int first) {
+        win_first = first;
+        const long long key0 = (long long)(first + lane) * ps;
+        win = key0 < k_hi ? __ldg(table + first + lane) : 0;
     };
-    const auto stage = [&](int tile, long long off) {
+    if (ntiles > 0) fill_window(win_first);
+    // a key's row in its page, -1 on a bad page number (uniform arguments: the window may move)
+    const auto row_at = [&](int key, int page) -> long long {
+        if ((unsigned)page >= (unsigned)p.pg.n_pages) {
+            set_status(p.pg.status);
+            return -1;
+        }
+        return (long long)page * p.pg.page_stride + (long long)(key % ps) * p.pg.slot_stride;
+    };
+    const long long lane_off = (long long)(lane / CH) * p.pg.slot_stride + (lane % CH) * 8;
+    const auto stage = [&](int tile) {
         const uint32_t ks = ring + (uint32_t)((tile / kRowsWarps) % kRowsStages) * 2 * kRowsTileBytes;
         const uint32_t vs = ks + kRowsTileBytes;
-        if (tile < ntiles) {
+        const int key0 = k_lo + tile * KT;
+        if (tile < ntiles && whole_tiles) {
+            const int pi = key0 / ps;
+            if (pi > win_first + 31) fill_window(pi);
+            const long long row = row_at(key0, __shfl_sync(0xffffffffu, win, pi - win_first));
+            const TC *kp = kb + (row < 0 ? 0 : row + lane_off), *vp = vb + (row < 0 ? 0 : row + lane_off);
+            const long long step = row < 0 ? 0 : 32 / CH * p.pg.slot_stride;
+            const int left = row < 0 ? 0 : k_hi - key0 - lane / CH;    // of the lane's rows, every 32 / CH-th
 #pragma unroll
             for (int i = 0; i < KT * CH / 32; ++i) {
-                const int idx = i * 32 + lane, r = idx / CH, c = idx - r * CH;
-                const long long o = __shfl_sync(0xffffffffu, off, r);
-                const bool on = o >= 0;
-                cp16_zfill(ks + rows_off<HD>(r, c), kb + (on ? o : 0) + c * 8, on);
-                cp16_zfill(vs + rows_off<HD>(r, c), vb + (on ? o : 0) + c * 8, on);
+                const uint32_t at = rows_off<HD>(i * (32 / CH) + lane / CH, lane % CH);
+                const bool on = i * (32 / CH) < left;
+                cp16_zfill(ks + at, on ? kp + i * step : kb, on);
+                cp16_zfill(vs + at, on ? vp + i * step : vb, on);
+            }
+        } else if (tile < ntiles) {
+            const int key = min(key0 + min(lane, KT - 1), k_hi - 1), pi = key / ps, last = min(key0 + KT, k_hi) - 1;
+            if (last / ps > win_first + 31) fill_window(key0 / ps);
+            const long long row = row_at(key, __shfl_sync(0xffffffffu, win, pi - win_first));
+#pragma unroll
+            for (int i = 0; i < KT * CH / 32; ++i) {
+                const int r = i * (32 / CH) + lane / CH;
+                const long long o = __shfl_sync(0xffffffffu, row, r);
+                const uint32_t at = rows_off<HD>(r, lane % CH);
+                const bool on = o >= 0 && key0 + r < k_hi;
+                cp16_zfill(ks + at, on ? kb + o + lane % CH * 8 : kb, on);
+                cp16_zfill(vs + at, on ? vb + o + lane % CH * 8 : vb, on);
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    long long off = row_of(warp);
 #pragma unroll
-    for (int i = 0; i < kRowsStages - 1; ++i) {
-        stage(warp + i * kRowsWarps, off);
-        off = row_of(warp + (i + 1) * kRowsWarps);
-    }
+    for (int i = 0; i < kRowsStages - 1; ++i) stage(warp + i * kRowsWarps);
     // q fragments: tile rows gq and gq + 8 at dims 16 kk + 2 tq + {0, 1} and + 8
     uint32_t qa[KS][4];
     const int ra = row0 + gq, rb = kSplit ? ra : row0 + gq + 8;
@@ -386,8 +432,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps) k_pages_rows(PagesAttention p
     for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     for (int tile = warp; tile < ntiles; tile += kRowsWarps) {
-        stage(tile + (kRowsStages - 1) * kRowsWarps, off);
-        off = row_of(tile + kRowsStages * kRowsWarps);
+        stage(tile + (kRowsStages - 1) * kRowsWarps);
         asm volatile("cp.async.wait_group %0;" ::"n"(kRowsStages - 1) : "memory");
         __syncwarp();
         const uint32_t ks = ring + (uint32_t)((tile / kRowsWarps) % kRowsStages) * 2 * kRowsTileBytes;
@@ -536,53 +581,83 @@ __global__ void __launch_bounds__(32 * kRowsWarps) k_pages_rows(PagesAttention p
     }
 }
 
-// The key ranges' partials of every (token, head), in slot order: a warp each, lane = HD / 32 dims.
+// The key ranges' partials of a (token, head): a CTA, warp w the slots w, w + 4, .., lane = HD / 32 dims. Every
+// slot's (m, l) is read at once, so that the partials' loads depend on nothing else and 8 a lane are on their
+// way; a slot without weight (a range that does not exist) is passed over. The warps' sums are added in order.
+constexpr int kMergeWarps = 4;
+constexpr int kMergeSlots = 4 * kPagesMaxSplits;
 template <int HD, typename TQ>
-__global__ void __launch_bounds__(128) k_pages_merge(PagesAttention p, PagesPlan pl) {
-    constexpr int DL = HD / 32;
+__global__ void __launch_bounds__(32 * kMergeWarps) k_pages_merge(PagesAttention p, PagesPlan pl) {
+    constexpr int DL = HD / 32, NS = kMergeSlots / 32, BATCH = 8;
+    __shared__ float s_w[kMergeSlots];
+    __shared__ float s_acc[kMergeWarps][HD];
     const PageBatchView &ba = p.ba;
-    const int lane = threadIdx.x & 31;
-    const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int t = (int)(w / p.nh), h = (int)(w - (long long)t * p.nh);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int t = blockIdx.x / p.nh, h = blockIdx.x - t * p.nh;
     if (t >= total_rows(ba)) return;
-    int n_own = 0;
-    if (pl.own_splits > 0) {
-        const int b = find_request(ba, t, lane);
-        int chunk;
-        own_chunks(own_len(p, b, lane), pl.own_splits, chunk, n_own);
+    griddep_wait();
+    const long long step = (long long)ba.T * p.nh, at = blockIdx.x;
+    float2 ml[NS];
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const int s = 32 * i + lane;
+        ml[i] = make_float2(-INFINITY, 0.f);
+        if (s < pl.slots) ml[i] = *reinterpret_cast<const float2 *>(pl.ml + (s * step + at) * 2);
+        M = fmaxf(M, ml[i].x);
     }
-    const int n = pl.prefix_slots + (n_own << pl.own_alt);
-    const long long step = (long long)ba.T * p.nh, at = (long long)t * p.nh + h;
-    float M = -INFINITY;
-    for (int s = lane; s < n; s += 32) M = fmaxf(M, pl.ml[(s * step + at) * 2]);
     M = warp_max(M);
     const float Ms = M == -INFINITY ? 0.f : M;
-    float L = 0.f, acc[DL];
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const float f = exp2_approx(ml[i].x - Ms);
+        L = fmaf(ml[i].y, f, L);
+        if (warp == 0) s_w[32 * i + lane] = f;
+    }
+    L = warp_sum(L);                                         // the same bits in every warp
+    __syncthreads();
+    float acc[DL];
 #pragma unroll
     for (int d = 0; d < DL; ++d) acc[d] = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < n; ++s) {
-        const float2 ml = __ldg(reinterpret_cast<const float2 *>(pl.ml + (s * step + at) * 2));
-        const float *src = pl.acc + (s * step + at) * HD + lane * DL;
-        const float f = exp2_approx(ml.x - Ms);
-        L = fmaf(ml.y, f, L);
-        if constexpr (DL == 4) {
-            const float4 v = __ldg(reinterpret_cast<const float4 *>(src));
-            acc[0] = fmaf(v.x, f, acc[0]);
-            acc[1] = fmaf(v.y, f, acc[1]);
-            acc[2] = fmaf(v.z, f, acc[2]);
-            acc[3] = fmaf(v.w, f, acc[3]);
-        } else {
-            const float2 v = __ldg(reinterpret_cast<const float2 *>(src));
-            acc[0] = fmaf(v.x, f, acc[0]);
-            acc[1] = fmaf(v.y, f, acc[1]);
-        }
-    }
-    const float inv = L > 0.f ? 1.f / L : 0.f;
-    TQ *dst = reinterpret_cast<TQ *>(p.out) + (long long)t * p.out_stride + h * HD + lane * DL;
+    for (int s0 = warp; s0 < pl.slots; s0 += kMergeWarps * BATCH) {
+        float f[BATCH], v[BATCH][DL];
 #pragma unroll
-    for (int d = 0; d < DL; ++d) dst[d] = from_float<TQ>(L == L ? acc[d] * inv : L);
-    if (p.lse && lane == 0) p.lse[at] = row_lse(M, L);
+        for (int i = 0; i < BATCH; ++i) {
+            const int s = s0 + kMergeWarps * i;
+            f[i] = s < pl.slots ? s_w[s] : 0.f;
+#pragma unroll
+            for (int d = 0; d < DL; ++d) v[i][d] = 0.f;
+            if (!(f[i] == 0.f)) {
+                const float *src = pl.acc + (s * step + at) * HD + lane * DL;
+                if constexpr (DL == 4) {
+                    const float4 x = *reinterpret_cast<const float4 *>(src);
+                    v[i][0] = x.x;
+                    v[i][1] = x.y;
+                    v[i][2] = x.z;
+                    v[i][3] = x.w;
+                } else {
+                    const float2 x = *reinterpret_cast<const float2 *>(src);
+                    v[i][0] = x.x;
+                    v[i][1] = x.y;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i)
+#pragma unroll
+            for (int d = 0; d < DL; ++d) acc[d] = fmaf(v[i][d], f[i], acc[d]);
+    }
+#pragma unroll
+    for (int d = 0; d < DL; ++d) s_acc[warp][lane * DL + d] = acc[d];
+    __syncthreads();
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    for (int d = threadIdx.x; d < HD; d += 32 * kMergeWarps) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kMergeWarps; ++w) v += s_acc[w][d];
+        reinterpret_cast<TQ *>(p.out)[(long long)t * p.out_stride + h * HD + d] = from_float<TQ>(L == L ? v * inv : L);
+    }
+    if (p.lse && threadIdx.x == 0) p.lse[at] = row_lse(M, L);
 }
 
 // Which kernel takes what. k_pages_tc pads a row tile to 128 rows and needs an SM to itself;
@@ -590,6 +665,10 @@ __global__ void __launch_bounds__(128) k_pages_merge(PagesAttention p, PagesPlan
 constexpr int kSms = 148;
 constexpr int kTcMinRows = 32;
 constexpr int kTcMinOwnRows = 64;
+// measured on k_pages_tc: a CTA's start and end, a key tile of two row tiles, of one (the alternate walk), and
+// k_pages_rows' rate over own keys
+constexpr double kTcFixedUs = 8.0, kTcTileUs = 1.8, kTcAltTileUs = 1.0, kOwnBytesPerUs = 4.5e6;
+constexpr int kOwnCtas = 8 * kSms;           // k_pages_rows' CTAs over own keys: requests differ in length
 PagesPlan plan_attention(const PagesAttention &p) {
     PagesPlan pl{};
     const PageBatchView &ba = p.ba;
@@ -608,20 +687,36 @@ PagesPlan plan_attention(const PagesAttention &p) {
     const auto splits = [&](long long ctas, long long want, long long keys) {   // key ranges that fill the GPU
         return std::min<long long>({std::max<long long>(1, want / ctas), up(keys, kPagesOwnKeys), kPagesMaxSplits});
     };
-    if (ba.prefix_len > 0) {
-        pl.prefix_tc = fits && rows > kTcMinRows;
-        pl.prefix_alt = pl.prefix_tc && (f32 || rows <= 128);
-        pl.prefix_tiles = (int)up(rows, !pl.prefix_tc ? rt : pl.prefix_alt ? 128 : 256);
-        const long long n = splits((long long)pl.prefix_tiles * nkv, pl.prefix_tc ? kSms : 2 * kSms, ba.prefix_len);
-        pl.prefix_chunk = (int)(up(up(ba.prefix_len, n), kPagesGrain) * kPagesGrain);
-        pl.prefix_splits = (int)up(ba.prefix_len, pl.prefix_chunk);
-        pl.prefix_slots = pl.prefix_splits << pl.prefix_alt;
-    }
     if (bound > 0) {
         pl.own_tc = fits && own_rows > kTcMinOwnRows;
         pl.own_alt = pl.own_tc && (f32 || own_rows <= 128);
         pl.own_tiles = (int)up(own_rows, !pl.own_tc ? rt : pl.own_alt ? 128 : 256);
-        pl.own_splits = (int)splits((long long)ba.B * pl.own_tiles * nkv, pl.own_tc ? kSms : 2 * kSms, bound);
+        pl.own_splits = (int)splits((long long)ba.B * pl.own_tiles * nkv, pl.own_tc ? kSms : kOwnCtas, bound);
+    }
+    if (ba.prefix_len > 0) {
+        pl.prefix_tc = fits && rows > kTcMinRows;
+        pl.prefix_alt = pl.prefix_tc && (f32 || rows <= 128);
+        pl.prefix_tiles = (int)up(rows, !pl.prefix_tc ? rt : pl.prefix_alt ? 128 : 256);
+        const long long row_ctas = (long long)pl.prefix_tiles * nkv;
+        long long n = splits(row_ctas, pl.prefix_tc ? kSms : 2 * kSms, ba.prefix_len);
+        if (pl.prefix_tc) {
+            // k_pages_tc shares the GPU with the own keys' kernel: the fewest ranges that take no longer than
+            // both kernels' work spread over all SMs (in us; own keys: half the tables' capacity)
+            const double own_us = pl.own_tc ? 0.0 : 0.5 * (double)(ba.B * bound) * nkv * p.pg.hd * 4 * pl.own_tiles / kOwnBytesPerUs;
+            const double tiles = (double)up(ba.prefix_len, 128), tile_us = pl.prefix_alt ? kTcAltTileUs : kTcTileUs;
+            double best = 1e30;
+            for (long long k = n, most = n; k >= 1; --k) {
+                const double t = kTcFixedUs + std::ceil(tiles / k) * tile_us;
+                const double all = std::max(t, (double)(k * row_ctas) / kSms * t + own_us);
+                if (all <= best * (k == most ? 1.0 : 0.999)) {
+                    best = all;
+                    n = k;
+                }
+            }
+        }
+        pl.prefix_chunk = (int)(up(up(ba.prefix_len, n), kPagesGrain) * kPagesGrain);
+        pl.prefix_splits = (int)up(ba.prefix_len, pl.prefix_chunk);
+        pl.prefix_slots = pl.prefix_splits << pl.prefix_alt;
     }
     pl.slots = pl.prefix_slots + (pl.own_splits << pl.own_alt);
     return pl;
@@ -632,6 +727,7 @@ size_t plan_bytes(const PagesAttention &p, const PagesPlan &pl) {
 
 template <int HD, typename TQ, typename TC>
 cudaError_t attention_typed(const PagesAttention &p, PagesPlan pl, cudaStream_t s) {
+    const int nkv = p.pg.nkv;
     pl.acc = static_cast<float *>(p.ws);
     pl.ml = pl.acc + (size_t)pl.slots * p.ba.T * p.nh * HD;
     if (pl.prefix_tc || pl.own_tc) {
@@ -642,10 +738,19 @@ cudaError_t attention_typed(const PagesAttention &p, PagesPlan pl, cudaStream_t 
                       (pl.own_tc ? 0 : p.ba.B * pl.own_tiles * pl.own_splits);
     cudaError_t e = raise_smem(k_pages_rows<HD, TQ, TC>, kRowsSmem);
     if (e != cudaSuccess) return e;
-    if (items > 0) k_pages_rows<HD, TQ, TC><<<dim3(items, p.pg.nkv), 32 * kRowsWarps, kRowsSmem, s>>>(p, pl);
-    if (pl.slots != 1)
-        k_pages_merge<HD, TQ><<<(unsigned)(((long long)p.ba.T * p.nh + 3) / 4), 128, 0, s>>>(p, pl);
-    return cudaGetLastError();
+    // k_pages_rows does not read what k_pages_tc writes: it starts beside it (and ends after it, which is what
+    // the join waits for)
+    if (items > 0) {
+        if (pl.prefix_tc || pl.own_tc)
+            e = launch_dependent(k_pages_rows<HD, TQ, TC>, dim3(items + 1, nkv), 32 * kRowsWarps, kRowsSmem, s, p, pl);
+        else
+            k_pages_rows<HD, TQ, TC><<<dim3(items, nkv), 32 * kRowsWarps, kRowsSmem, s>>>(p, pl);
+    }
+    if (e == cudaSuccess) e = cudaGetLastError();
+    if (e == cudaSuccess && pl.slots != 1)
+        e = launch_dependent(k_pages_merge<HD, TQ>, dim3((unsigned)(p.ba.T * p.nh)),
+                             32 * kMergeWarps, 0, s, p, pl);
+    return e;
 }
 
 }  // namespace

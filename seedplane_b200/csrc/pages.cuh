@@ -88,16 +88,6 @@ SP_DEVINL int own_len(const PagesAttention &p, int b, int lane) {
     }
     return len;
 }
-// element offset of a key's row in its page, -1 on a bad page number
-SP_DEVINL long long page_row(const PagesView &pg, const int *table, int key) {
-    const int pi = key / pg.page_size, page = table[pi];
-    if ((unsigned)page >= (unsigned)pg.n_pages) {
-        set_status(pg.status);
-        return -1;
-    }
-    return (long long)page * pg.page_stride + (long long)(key - pi * pg.page_size) * pg.slot_stride;
-}
-
 // ---- key ranges --------------------------------------------------------------------------------
 constexpr int kPagesGrain = 128;                             // key ranges are multiples of this
 constexpr int kPagesOwnKeys = 256;                           // own keys per range at least

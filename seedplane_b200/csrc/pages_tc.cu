@@ -97,6 +97,12 @@ SP_DEVINL float max3(float a, float b, float c) {             // NaN is passed o
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
+SP_DEVINL void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+SP_DEVINL void bulk_s2g(void *dst, uint32_t src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
 SP_DEVINL bool elect_one() {
     uint32_t p;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
@@ -156,6 +162,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const PageBatchView &ba = p.ba;
     const int g = blockIdx.y, G = p.nh / p.pg.nkv;
+    griddep_launch_dependents();
+    if (warp == kTcProducer && lane == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_k)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_v)) : "memory");
+    }
     // the item
     const int total = total_rows(ba);
     int q0 = 0, row0, nrows, slot = 0, own0 = INT_MAX / 2, own_tile0 = INT_MAX, item = blockIdx.x;
@@ -199,8 +210,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         } else {
             int chunk, parts;
             own_chunks(len, pl.own_splits, chunk, parts);
-            if (z >= parts) return;
             slot = pl.prefix_slots + (z << pl.own_alt);
+            if (z >= parts) {                // no such range: nothing to join
+                for (int i = tid; i < nrows << pl.own_alt; i += kTcThreads) {
+                    const int k = i / nrows, row = row0 + i - k * nrows;
+                    const long long at = ((long long)(slot + k) * ba.T + q0 + row / G) * p.nh + g * G + row % G;
+                    *reinterpret_cast<float2 *>(pl.ml + at * 2) = make_float2(-INFINITY, 0.f);
+                }
+                return;
+            }
             ks.table_a = table;
             ks.lo_a = z * chunk;
             ks.hi_a = min(ks.lo_a + chunk, last);
@@ -238,32 +256,41 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     tc_fence_after();
     const uint32_t tmem = s_tmem;
 
-    // 384 threads of 168 registers at launch: the softmax groups take 224, the third 56 (the sum is the same)
+    // 384 threads of 168 registers at launch: the softmax groups take 216, the third 72 (the sum is the same; with
+    // 56 the MMA warp spilled, 188 -> 212 us)
     if (warp >= kTcProducer) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == kTcProducer) {
         // ring order: K of the first `lead` tiles, then V of tile i and K of tile i + lead
         const int lead = alt ? 2 : 1;
         int it = 0, tails = 0;
-        const auto load = [&](int i, bool is_v) -> bool {
-            const int st = it % kTcStages;
-            if (it >= kTcStages && !w.wait_warp(&bar.empty[st], (uint32_t)(it / kTcStages - 1) & 1u)) return false;
-            const int lo = ks.lo(i), keys = min(kTcKeys, ks.hi(i) - lo);
+        // the page numbers around K's and V's places in the sequence, 32 at a time: a tile's are at hand before
+        // its stage is free
+        struct Window {
+            int pages, first = INT_MIN, seg = -1;
+        } win_k, win_v;
+        const auto load = [&](int i, bool is_v, Window &win) -> bool {
+            const int st = it % kTcStages, lo = ks.lo(i), hi = ks.hi(i), keys = min(kTcKeys, hi - lo);
             const int per = min(p.pg.page_size, kTcKeys), pages = (keys + per - 1) / per;
+            const int seg = i >= ks.n_a, first = lo / p.pg.page_size;
+            if (seg != win.seg || first < win.first || first + (pages - 1) * per / p.pg.page_size > win.first + 31) {
+                win.seg = seg;
+                win.first = first;
+                const int pi = first + lane;
+                win.pages = (long long)pi * p.pg.page_size < hi ? __ldg(ks.table(i) + pi) : 0;
+            }
+            // lane: box `lane` of the tile (a page, or 128 slots of a larger one)
+            const int key = lo + min(lane, pages - 1) * per, pi = key / p.pg.page_size;
+            int page = __shfl_sync(0xffffffffu, win.pages, pi - win.first);
+            const int slot0 = key - pi * p.pg.page_size;
+            if ((unsigned)page >= (unsigned)p.pg.n_pages) {
+                if (lane < pages) set_status(p.pg.status);
+                page = p.pg.n_pages;         // outside the tensor: zeros
+            }
+            if (it >= kTcStages && !w.wait_warp(&bar.empty[st], (uint32_t)(it / kTcStages - 1) & 1u)) return false;
             const uint32_t dst = ring + (uint32_t)st * L::kTile;
             const bool tail = is_v && keys < kTcKeys;
             uint64_t *b = tail ? &bar.tail : &bar.full[st];
-            int page = 0, slot0 = 0;
-            if (lane < pages) {
-                const int key = lo + lane * per;
-                const int pi = key / p.pg.page_size;
-                page = ks.table(i)[pi];
-                slot0 = key - pi * p.pg.page_size;
-                if ((unsigned)page >= (unsigned)p.pg.n_pages) {
-                    set_status(p.pg.status);
-                    page = p.pg.n_pages;     // outside the tensor: zeros
-                }
-            }
             if (lane == 0) mbar_arrive_expect_tx(b, (uint32_t)(pages * per) * HD * 2);
             __syncwarp();
             if (lane < pages) {
@@ -289,7 +316,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         int kc = 0, vc = 0;
         for (bool ok = true; ok && vc < n;) {
             const bool is_v = kc >= n || kc >= vc + lead;
-            ok = load(is_v ? vc : kc, is_v);
+            ok = is_v ? load(vc, true, win_v) : load(kc, false, win_k);
             ++(is_v ? vc : kc);
         }
         // no copy is in flight when the CTA ends, whoever gave up
@@ -391,39 +418,47 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         __syncwarp();
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int grp = warp >> 2;
         const TQ *qbase = reinterpret_cast<const TQ *>(p.q);
-        // Q rows into swizzled tiles (rows behind the last: zero)
-        const int fill = (alt || nq == 1 ? 1 : 2) * kTcRows;
-        for (int i = tid; i < fill * CH; i += 256) {
-            const int r = i / CH, c = i - r * CH;
-            const uint32_t at = base + (uint32_t)(r >> 7) * L::kTile + (c >> 3) * L::kHalf + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4);
-            const int row = row0 + r;
-            const TQ *src = qbase + (long long)(q0 + row / G) * p.q_stride + (g * G + row % G) * HD + c * 8;
-            uint4 v = make_uint4(0u, 0u, 0u, 0u), lo = v;
-            if (r < nrows) {
+        // Q rows into swizzled tiles (rows behind the last: zero), a batch of loads under way at once
+        const int fill = (alt || nq == 1 ? 1 : 2) * kTcRows * CH;
+        constexpr int QB = kSplit ? 4 : 8;
+        for (int i0 = tid; i0 < fill; i0 += 256 * QB) {
+            uint4 v[QB], v2[kSplit ? QB : 1];
+#pragma unroll
+            for (int j = 0; j < QB; ++j) {
+                const int i = i0 + 256 * j, r = i / CH, c = i - r * CH, row = row0 + r;
+                v[j] = make_uint4(0u, 0u, 0u, 0u);
+                if constexpr (kSplit) v2[j] = v[j];
+                if (r < nrows) {
+                    const TQ *src = qbase + (long long)(q0 + row / G) * p.q_stride + (g * G + row % G) * HD + c * 8;
+                    v[j] = __ldg(reinterpret_cast<const uint4 *>(src));
+                    if constexpr (kSplit) v2[j] = __ldg(reinterpret_cast<const uint4 *>(src) + 1);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < QB; ++j) {
+                const int i = i0 + 256 * j, r = i / CH, c = i - r * CH;
+                if (i >= fill) break;
+                const uint32_t at = base + (uint32_t)(r >> 7) * L::kTile + (c >> 3) * L::kHalf + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4);
                 if constexpr (kSplit) {
-                    const float4 a = *reinterpret_cast<const float4 *>(src), b = *(reinterpret_cast<const float4 *>(src) + 1);
-                    const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                    const uint32_t x[8] = {v[j].x, v[j].y, v[j].z, v[j].w, v2[j].x, v2[j].y, v2[j].z, v2[j].w};
                     uint32_t hw[4], lw[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
+                        const float x0 = __uint_as_float(x[2 * k]), x1 = __uint_as_float(x[2 * k + 1]);
                         float h0, h1;
-                        hw[k] = pack2<TC>(x[2 * k], x[2 * k + 1]);
+                        hw[k] = pack2<TC>(x0, x1);
                         unpack2<TC>(hw[k], h0, h1);
-                        lw[k] = pack2<TC>(x[2 * k] - h0, x[2 * k + 1] - h1);
+                        lw[k] = pack2<TC>(x0 - h0, x1 - h1);
                     }
-                    v = make_uint4(hw[0], hw[1], hw[2], hw[3]);
-                    lo = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+                    st_shared16(at, hw[0], hw[1], hw[2], hw[3]);
+                    st_shared16(at + L::kTile, lw[0], lw[1], lw[2], lw[3]);
                 } else {
-                    v = *reinterpret_cast<const uint4 *>(src);
+                    st_shared16(at, v[j].x, v[j].y, v[j].z, v[j].w);
                 }
             }
-            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-            if constexpr (kSplit)
-                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at + L::kTile), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w)
-                             : "memory");
         }
         fence_proxy_async_smem();
         mbar_arrive(&bar.q_full);
@@ -507,13 +542,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 tc_fence_before();
                 mbar_arrive(&bar.p_full[grp]);
             }
-            // O and the row's statistics
-            if (any && ok) ok = w.wait_warp(&bar.o_full[grp], 0);
+            // O and the row's statistics. A thread's row goes through shared memory (the tiles are done with once both
+            // groups' products are) and out as one bulk copy: 16-byte stores of 32 rows a warp took 4 us
+            for (int q = 0; q < nq; ++q)
+                if (ok && (alt ? q < n : n > 0)) ok = w.wait_warp(&bar.o_full[q], 0);
             tc_fence_after();
             const long long rt = q0 + row / G, hh = g * G + row % G;
             const long long at = ((long long)(slot + (alt ? grp : 0)) * ba.T + rt) * p.nh + hh;
             const bool direct = pl.slots == 1;
             const float inv = l > 0.f ? 1.f / l : 0.f;
+            const uint32_t stage = base + (uint32_t)(grp * kTcRows + (warp & 3) * 32 + lane) * (HD * 4 + 16);
 #pragma unroll
             for (int k = 0; k < HD / 32; ++k) {
                 uint32_t o[32];
@@ -524,36 +562,34 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
                     for (int j = 0; j < 32; ++j) o[j] = 0u;
                 }
-                if (live && direct) {
-                    TQ *dst = reinterpret_cast<TQ *>(p.out) + rt * p.out_stride + hh * HD + 32 * k;
-                    float v[32];
+                if (direct) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = l == l ? __uint_as_float(o[j]) * inv : l;
-                    if constexpr (kSplit) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            reinterpret_cast<float4 *>(dst)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            reinterpret_cast<uint4 *>(dst)[j] =
-                                make_uint4(pack2<TQ>(v[8 * j], v[8 * j + 1]), pack2<TQ>(v[8 * j + 2], v[8 * j + 3]),
-                                           pack2<TQ>(v[8 * j + 4], v[8 * j + 5]), pack2<TQ>(v[8 * j + 6], v[8 * j + 7]));
-                    }
-                } else if (live) {
-                    uint4 *dst = reinterpret_cast<uint4 *>(pl.acc + at * HD + 32 * k);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) dst[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                    for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(l == l ? __uint_as_float(o[j]) * inv : l);
                 }
-                __syncwarp();
+                if (direct && !kSplit) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t v[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[i] = pack2<TC>(__uint_as_float(o[8 * j + 2 * i]), __uint_as_float(o[8 * j + 2 * i + 1]));
+                        st_shared16(stage + 64 * k + 16 * j, v[0], v[1], v[2], v[3]);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) st_shared16(stage + 128 * k + 16 * j, o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                }
             }
+            fence_proxy_async_smem();
             if (live) {
                 if (direct) {
+                    bulk_s2g(reinterpret_cast<TQ *>(p.out) + rt * p.out_stride + hh * HD, stage, HD * sizeof(TQ));
                     if (p.lse) p.lse[rt * p.nh + hh] = row_lse(m, l);
                 } else {
+                    bulk_s2g(pl.acc + at * HD, stage, HD * 4);
                     *reinterpret_cast<float2 *>(pl.ml + at * 2) = make_float2(m, l);
                 }
             }
+            asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
             tc_fence_before();
         }
     }
