@@ -297,6 +297,25 @@ int sp_pages_attention(int device, const sp_pages *pages, const sp_page_batch *b
                        int32_t dtype, int64_t q_stride, float scale, void *out_dev, int64_t out_stride, float *lse_dev,
                        void *workspace_dev, int64_t workspace_bytes, void *stream);
 
+/* One packed pass of a ragged batch through the model over pages: row i of the batch is token
+ * tokens_dev[i] (int32, on the engine's device), its K / V go to its request's pages (sp_pages_append) and it
+ * attends to the shared prefix and its request's own keys (sp_pages_attention), at RoPE position
+ * prefix_len + own key. layer_pages: HOST array of the engine's `layers` entries, SP_F16, with the engine's
+ * kv_heads and head_dim (their status_dev is not used: sp_device_status reports). argmax_dev int32 [batch]:
+ * the greedy token after each request's last row; logits_dev: NULL or fp32 [batch][vocab]. Every request
+ * has at least one row; batch 1 .. 256, tokens 1 .. 512 (and exactly q_start[batch]). Like sp_prefill_batch
+ * and sp_decode_batch, for caches that share a prefix. The engine's workspace is used. */
+int sp_forward_pages(sp_engine *e, const sp_pages *layer_pages, const sp_page_batch *batch, const int32_t *tokens_dev,
+                     float *logits_dev, int32_t *argmax_dev, void *stream);
+
+/* Greedy decode of a batch over pages, fed back on the device: n_steps passes of one row per request. On
+ * entry tokens_dev[batch] (int32, device) holds each request's next token and lens_dev its own keys so far;
+ * every step appends the token (lens_dev[b] += 1) and replaces it by its argmax, also stored at
+ * out_tokens_dev[step][batch]. batch->lens_dev and tokens_dev are written; batch->q_start_dev must be NULL,
+ * max_q 1, tokens = batch <= 64; the tables must have room for the steps. */
+int sp_decode_pages(sp_engine *e, const sp_pages *layer_pages, const sp_page_batch *batch, int32_t *tokens_dev,
+                    int32_t n_steps, int32_t *out_tokens_dev, void *stream);
+
 /* Bytes of workspace sp_accept_chains needs, or SP_ERR_*. */
 int64_t sp_accept_chains_workspace(int32_t batch, int32_t drafts, int32_t vocab);
 

@@ -27,6 +27,7 @@ EXPORTED = ("sp_last_error", "sp_version", "sp_engine_create", "sp_engine_destro
             "sp_forward", "sp_decode", "sp_decode_batch", "sp_prefill_batch", "sp_verify_tree", "sp_kv_commit", "sp_kv_copy", "sp_argmax", "sp_argmax_noalloc", "sp_mcol_gemm", "sp_topk",
             "sp_accept_stochastic", "sp_accept_greedy", "sp_sample_filter",
             "sp_pages_append", "sp_pages_attention", "sp_pages_attention_workspace",
+            "sp_forward_pages", "sp_decode_pages",
             "sp_accept_chains", "sp_accept_chains_workspace",
             "sp_device_status",
             "sp_trace_read")
@@ -111,6 +112,8 @@ def load(path: Path = LIB_PATH):
         "sp_pages_attention_workspace": (i64, [C.POINTER(SpPages), C.POINTER(SpPageBatch), i32, i32]),
         "sp_pages_attention": (C.c_int, [C.c_int, C.POINTER(SpPages), C.POINTER(SpPageBatch), i32, vp, i32, i64,
                                          C.c_float, vp, i64, vp, vp, i64, vp]),
+        "sp_forward_pages": (C.c_int, [vp, C.POINTER(SpPages), C.POINTER(SpPageBatch), vp, vp, vp, vp]),
+        "sp_decode_pages": (C.c_int, [vp, C.POINTER(SpPages), C.POINTER(SpPageBatch), vp, i32, vp, vp]),
         "sp_accept_chains_workspace": (i64, [i32, i32, i32]),
         "sp_accept_chains": (C.c_int, [C.c_int, i32, i32, i32, vp, i64, i64, vp, i64, i64, i32, vp, vp, vp, vp, vp, vp,
                                        vp, i64, vp]),

@@ -20,6 +20,7 @@ import torch
 
 MAX_BATCH = 64                          # requests per sp_decode_batch call
 MAX_PREFILL_BATCH = 256                 # prompts per sp_prefill_batch call
+MAX_PASS_TOKENS = 512                   # rows of a packed pass over pages (sp_forward_pages)
 
 
 def generate_batch(engine, prompts: Sequence[Sequence[int]], max_new_tokens, stop: Iterable[int] = (),
@@ -77,3 +78,85 @@ def generate_batch(engine, prompts: Sequence[Sequence[int]], max_new_tokens, sto
         if own:
             for kv in kvs:
                 kv.close()
+
+
+def generate_shared(engine, prefix: Sequence[int], prompts: Sequence[Sequence[int]], max_new_tokens, stop: Iterable[int] = (),
+                    block: int = 16, page_size: int = 64, timer=None) -> List[List[int]]:
+    """`generate_batch` for requests that all start with `prefix`: the same greedy tokens as for the prompts
+    prefix + prompt, with the prefix run through the model once and its keys and values kept once, in pages that every
+    request reads (the attention of a step reads them once for the whole batch). Arguments as `generate_batch`; each
+    prompt has at least one token."""
+    from .paged import PageBatch
+    n_req = len(prompts)
+    if n_req == 0:
+        return []
+    limits = [int(max_new_tokens)] * n_req if isinstance(max_new_tokens, int) else [int(m) for m in max_new_tokens]
+    if len(limits) != n_req or any(m < 1 for m in limits):
+        raise ValueError("every request needs max_new_tokens >= 1")
+    prefix = [int(t) for t in prefix]
+    prompts = [[int(t) for t in p] for p in prompts]
+    if any(not p for p in prompts):
+        raise ValueError("empty prompt")
+    if len(prefix) + max(len(p) + m for p, m in zip(prompts, limits)) > engine.cfg.max_positions:
+        raise ValueError("a request exceeds the model's positions")
+    stops = {int(s) for s in stop}
+    dev = engine.device
+    int32 = lambda v: torch.tensor(v, dtype=torch.int32).to(dev)  # noqa: E731
+    need = [-(-(len(p) + m) // page_size) for p, m in zip(prompts, limits)]
+    n_prefix = -(-len(prefix) // page_size)
+    pages = engine.new_pages(n_prefix + sum(need), page_size)
+    prefix_table = torch.arange(n_prefix, dtype=torch.int32, device=dev)
+    tables = torch.zeros((n_req, max(need)), dtype=torch.int32)
+    at = n_prefix
+    for b, m in enumerate(need):
+        tables[b, :m] = torch.arange(at, at + m, dtype=torch.int32)
+        at += m
+    tables = tables.to(dev)
+    if timer:
+        timer(True)
+    for c0 in range(0, len(prefix), MAX_PASS_TOKENS):          # the prefix, as one request's own keys
+        part = prefix[c0:c0 + MAX_PASS_TOKENS]
+        one = PageBatch(prefix_table[None], int32([c0 + len(part)]), max_q=len(part))
+        engine.forward_pages(pages, one, int32(part))
+    shared = dict(prefix_table=prefix_table, prefix_len=len(prefix))
+    done_rows, firsts = [0] * n_req, [None] * n_req
+    b = 0
+    while b < n_req:                                           # prompts packed into passes; a long one in several
+        rows, room = [], MAX_PASS_TOKENS
+        while b < n_req and room > 0 and len(rows) < MAX_PREFILL_BATCH:
+            take = min(room, len(prompts[b]) - done_rows[b])
+            rows.append((b, done_rows[b], take))
+            done_rows[b] += take
+            room -= take
+            if done_rows[b] < len(prompts[b]):
+                break
+            b += 1
+        flat = [t for r, r0, take in rows for t in prompts[r][r0:r0 + take]]
+        starts = [0]
+        for _, _, take in rows:
+            starts.append(starts[-1] + take)
+        part = PageBatch(tables[rows[0][0]:rows[-1][0] + 1], int32([r0 + take for _, r0, take in rows]), q_start=int32(starts),
+                         tokens=len(flat), max_q=max(take for _, _, take in rows), **shared)
+        argmax, _ = engine.forward_pages(pages, part, int32(flat))
+        for j, (r, r0, take) in enumerate(rows):
+            if r0 + take == len(prompts[r]):
+                firsts[r] = argmax[j]
+    out = [[t] for t in torch.stack(firsts).cpu().tolist()]
+    done = [o[0] in stops or m == 1 for o, m in zip(out, limits)]
+    while not all(done):
+        active = [b for b in range(n_req) if not done[b]]
+        for c0 in range(0, len(active), MAX_BATCH):
+            group = active[c0:c0 + MAX_BATCH]
+            n = max(1, min(block, min(limits[b] - len(out[b]) for b in group)))
+            step = PageBatch(tables[int32(group).long()], int32([len(prompts[b]) + len(out[b]) - 1 for b in group]), **shared)
+            rows = engine.decode_pages(pages, step, int32([out[b][-1] for b in group]), n).cpu().tolist()
+            for j, b in enumerate(group):
+                for i in range(n):
+                    out[b].append(rows[i][j])
+                    if rows[i][j] in stops or len(out[b]) >= limits[b]:
+                        done[b] = True
+                        break
+    if timer:
+        timer(False)
+    engine.status()
+    return out

@@ -179,6 +179,8 @@ struct sp_engine {
     int32_t *last_only_buf = nullptr;       // sp_forward(all_logits = 2) through the step path: per-step argmaxes
     int32_t last_only_cap = 0;
     std::map<int, cudaGraphExec_t> bgraphs; // batched decode step per batch size
+    float *pg_ws = nullptr;                 // paged passes: attention workspace
+    size_t pg_ws_bytes = 0;
     int32_t *vt_argmax = nullptr;           // [kSmallNodes] argmax of a captured verify pass
     std::map<std::pair<sp_kv *, int>, cudaGraphExec_t> vgraphs;   // verify pass per (cache, nodes)
     unsigned long long *mc_trace = nullptr;  // SEEDPLANE_MCOL_TRACE: stamps of the last multi-column GEMM
@@ -1143,12 +1145,13 @@ void sp_engine_destroy(sp_engine *e) {
     for (auto &g : e->bgraphs) cudaGraphExecDestroy(g.second);
     cudaFree(e->bt);
     cudaFree(e->bp);
+    cudaFree(e->pg_ws);
     cudaFree(e->last_only_buf);
     delete e;
 }
 
 int64_t sp_engine_device_bytes(const sp_engine *e) {
-    return e ? (int64_t)(e->arena_bytes + e->ws_bytes + e->pf_bytes) : 0;
+    return e ? (int64_t)(e->arena_bytes + e->ws_bytes + e->pf_bytes + e->pg_ws_bytes) : 0;
 }
 
 int sp_kv_create(sp_engine *e, int32_t capacity, sp_kv **out) {
@@ -1940,6 +1943,113 @@ int sp_pages_attention(int device, const sp_pages *pages, const sp_page_batch *b
     OnDevice on;
     SP_CUDA(on.enter(device));
     SP_CUDA(launch_pages_attention(p, (cudaStream_t)stream));
+    return SP_OK;
+}
+
+// What the paged passes have in common: the checks, and the layers' parameter blocks without their pages.
+static int paged_pass_args(sp_engine *e, const sp_pages *layer_pages, const sp_page_batch *batch, PagesAppend &ap,
+                           PagesAttention &at) {
+    if (!e || !layer_pages || !batch) return fail(SP_ERR_INVALID, "null argument");
+    if (!e->prefill) return fail(SP_ERR_UNSUPPORTED, "paged passes need the batched pass (SEEDPLANE_PREFILL=steps)");
+    const sp_config &c = e->c;
+    for (int l = 0; l < c.layers; ++l) {
+        const sp_pages &pg = layer_pages[l];
+        if (pg.kv_heads != c.kv_heads || pg.head_dim != c.head_dim || pg.dtype != SP_F16)
+            return fail(SP_ERR_INVALID, "layer %d: pages of %d heads of %d, dtype %d, for fp16 pages of %d heads of %d", l,
+                        pg.kv_heads, pg.head_dim, pg.dtype, c.kv_heads, c.head_dim);
+        int rc = attention_args(&pg, batch, c.heads, SP_F32, at);
+        if (rc) return rc;
+    }
+    if (batch->batch < 1 || batch->batch > kPrefillBatchMax || batch->tokens < batch->batch || batch->tokens > kPrefillMaxTokens)
+        return fail(SP_ERR_CAPACITY, "a paged pass takes 1..%d requests of 1..%d rows together, not %d of %d", kPrefillBatchMax,
+                    kPrefillMaxTokens, batch->batch, batch->tokens);
+    if ((size_t)kPrefillMaxTokens * (2 * c.heads + 2 * c.kv_heads) * c.head_dim * sizeof(float) > kAttnPartBytes)
+        return fail(SP_ERR_UNSUPPORTED, "paged passes: %d heads of %d do not fit the pass's scratch", c.heads, c.head_dim);
+    if (batch->prefix_len >= c.max_positions)
+        return fail(SP_ERR_CAPACITY, "prefix of %d keys outside the RoPE table", batch->prefix_len);
+    ap.nh = c.heads;
+    ap.in_type = VT_F32;
+    ap.cache_type = VT_F16;
+    ap.rope = e->rope;
+    ap.rope_positions = c.max_positions;
+    ap.rot = c.head_dim;
+    ap.ba = at.ba;
+    at.scale = 1.0f / sqrtf((float)c.head_dim);
+    SP_CUDA(cudaSetDevice(e->device));
+    size_t need = 0;
+    for (int l = 0; l < c.layers; ++l) {                     // the plan depends on the pages' layout
+        int rc = attention_args(&layer_pages[l], batch, c.heads, SP_F32, at);
+        if (rc) return rc;
+        need = std::max(need, pages_attention_workspace(at));
+    }
+    if (e->pg_ws_bytes < need) {
+        if (e->pg_ws) {
+            SP_CUDA(cudaFree(e->pg_ws));                     // waits for the passes that use it
+            e->pg_ws = nullptr;
+            e->pg_ws_bytes = 0;
+        }
+        SP_CUDA(cudaMalloc(&e->pg_ws, need));
+        e->pg_ws_bytes = need;
+    }
+    at.ws = e->pg_ws;
+    return SP_OK;
+}
+
+static int paged_pass(sp_engine *e, const sp_pages *layer_pages, const sp_page_batch *batch, PagesAppend ap, PagesAttention at,
+                      const int32_t *tokens_dev, float *logits_dev, int32_t *argmax_dev, cudaStream_t s) {
+    const sp_config &c = e->c;
+    const int T = batch->tokens, B = batch->batch, QR = (c.heads + 2 * c.kv_heads) * c.head_dim;
+    float *y = e->pf.part, *o = y + (size_t)kPrefillMaxTokens * QR;
+    SP_CUDA(launch_prefill_embed(e->pf_dims, e->pf, e->embed, tokens_dev, T, e->st, s));
+    for (int l = 0; l < c.layers; ++l) {
+        const sp_pages &pg = layer_pages[l];
+        at.pg = PagesView{pg.k_dev, pg.v_dev, pg.page_stride, pg.head_stride, pg.slot_stride, pg.n_pages, pg.page_size,
+                          pg.kv_heads, pg.head_dim, &e->st->err};
+        ap.pg = at.pg;
+        SP_CUDA(launch_pages_layer_front(e->pf_dims, e->layers[l].pf, e->pf, ap, at, y, o, e->st, s));
+        SP_CUDA(launch_prefill_layer_ffn(e->pf_dims, e->layers[l].pf, e->pf, T, e->st, s));
+    }
+    PrefillScratch g = e->pf;
+    g.x = e->pf.q;                                           // free after the last layer's attention
+    SP_CUDA(launch_pages_last_rows(g.x, e->pf.x, at.ba, c.hidden, s));
+    for (int b0 = 0; b0 < B; b0 += kPrefillLogitRows) {
+        const int rows = std::min(kPrefillLogitRows, B - b0);
+        float *out = logits_dev ? logits_dev + (size_t)b0 * c.vocab : e->pf.logits;
+        SP_CUDA(launch_prefill_logits(e->pf_dims, g, e->final_norm, e->head_pf, b0, rows, out, e->st, s));
+        SP_CUDA(launch_argmax_rows(out, rows, c.vocab, c.vocab, argmax_dev + b0, e->am, s));
+    }
+    return SP_OK;
+}
+
+int sp_forward_pages(sp_engine *e, const sp_pages *layer_pages, const sp_page_batch *batch, const int32_t *tokens_dev,
+                     float *logits_dev, int32_t *argmax_dev, void *stream) {
+    PagesAppend ap{};
+    PagesAttention at{};
+    if (!tokens_dev || !argmax_dev) return fail(SP_ERR_INVALID, "null argument");
+    int rc = paged_pass_args(e, layer_pages, batch, ap, at);
+    if (rc) return rc;
+    return paged_pass(e, layer_pages, batch, ap, at, tokens_dev, logits_dev, argmax_dev, (cudaStream_t)stream);
+}
+
+int sp_decode_pages(sp_engine *e, const sp_pages *layer_pages, const sp_page_batch *batch, int32_t *tokens_dev,
+                    int32_t n_steps, int32_t *out_tokens_dev, void *stream) {
+    PagesAppend ap{};
+    PagesAttention at{};
+    if (!tokens_dev || !out_tokens_dev) return fail(SP_ERR_INVALID, "null argument");
+    if (n_steps <= 0) return fail(SP_ERR_INVALID, "n_steps must be positive");
+    if (batch && (batch->q_start_dev || batch->max_q != 1 || batch->tokens != batch->batch || batch->batch > kBatchMax))
+        return fail(SP_ERR_INVALID, "a decode batch has one row per request, no q_start, at most %d requests", kBatchMax);
+    int rc = paged_pass_args(e, layer_pages, batch, ap, at);
+    if (rc) return rc;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (!e->bt) SP_CUDA(cudaMalloc(&e->bt, sizeof(BatchIn)));
+    int32_t *lens = const_cast<int32_t *>(batch->lens_dev);
+    for (int i = 0; i < n_steps; ++i) {
+        SP_CUDA(launch_pages_advance(lens, tokens_dev, nullptr, nullptr, batch->batch, s));
+        rc = paged_pass(e, layer_pages, batch, ap, at, tokens_dev, nullptr, e->bt->argmax, s);
+        if (rc) return rc;
+        SP_CUDA(launch_pages_advance(lens, tokens_dev, e->bt->argmax, out_tokens_dev + (size_t)i * batch->batch, batch->batch, s));
+    }
     return SP_OK;
 }
 

@@ -491,6 +491,16 @@ struct PagesAttention {
 size_t pages_attention_workspace(const PagesAttention &p);
 cudaError_t launch_pages_attention(const PagesAttention &p, cudaStream_t s);
 
+// The front of a layer for a packed pass over pages (prefill.cu): RMSNorm, QKV GEMM, append (bias, rotation,
+// K / V into the layer's pages), attention, O GEMM (+= x). `ap` and `at` carry the batch, the pages and the head
+// counts; y fp32 [T][QKV rows] and o fp32 [T][heads * head_dim] are scratch.
+cudaError_t launch_pages_layer_front(const PrefillDims &d, const PrefillLayer &L, const PrefillScratch &s, PagesAppend ap,
+                                     PagesAttention at, float *y, float *o, DevState *st, cudaStream_t stream);
+// x_out row b = x row q_start[b + 1] - 1 (each request's last row), b < B
+cudaError_t launch_pages_last_rows(float *x_out, const float *x, const PageBatchView &ba, int H, cudaStream_t s);
+// a decode step's bookkeeping: before it (argmax null) lens[b] += 1; after it token b = argmax b, also to out
+cudaError_t launch_pages_advance(int32_t *lens, int32_t *tok, const int32_t *argmax, int32_t *out, int B, cudaStream_t s);
+
 // Verification of a batch's draft chains (chains.cu), as sp_accept_chains describes it.
 constexpr int kChainMaxDrafts = 64;
 struct ChainArgs {

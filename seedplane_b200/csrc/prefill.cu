@@ -727,6 +727,44 @@ __global__ void k_batch_advance(BatchLane *lanes, int32_t *tok, int32_t *pos, co
     lanes[b].slot = min(ns, lanes[b].cap - 1);
 }
 
+// fp16 hi / lo halves of fp32 values (a GEMM's input), four a thread
+__global__ void k_split_hilo(__half *xh, __half *xl, const float *x, long long n4) {
+    pdl_enter();
+    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= n4) return;
+    const float4 v = reinterpret_cast<const float4 *>(x)[i];
+    const float a[4] = {v.x, v.y, v.z, v.w};
+    uint32_t h[2], l[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const __half h0 = __float2half_rn(a[2 * k]), h1 = __float2half_rn(a[2 * k + 1]);
+        h[k] = h2bits(h0, h1);
+        l[k] = h2bits(__float2half_rn(a[2 * k] - __half2float(h0)), __float2half_rn(a[2 * k + 1] - __half2float(h1)));
+    }
+    reinterpret_cast<uint2 *>(xh)[i] = make_uint2(h[0], h[1]);
+    reinterpret_cast<uint2 *>(xl)[i] = make_uint2(l[0], l[1]);
+}
+
+__global__ void k_pages_last_rows(float *out, const float *x, PageBatchView ba, int H) {
+    pdl_enter();
+    const int b = blockIdx.x;
+    const int row = ba.q_start ? ba.q_start[b + 1] - 1 : (b + 1) * ba.max_q - 1;
+    const float *src = x + (size_t)min(max(row, 0), ba.T - 1) * H;
+    for (int j = threadIdx.x; j < H; j += blockDim.x) out[(size_t)b * H + j] = src[j];
+}
+
+__global__ void k_pages_advance(int32_t *lens, int32_t *tok, const int32_t *argmax, int32_t *out, int B) {
+    pdl_enter();
+    const int b = blockIdx.x * blockDim.x + threadIdx.x;
+    if (b >= B) return;
+    if (argmax) {
+        tok[b] = argmax[b];
+        out[b] = argmax[b];
+    } else {
+        lens[b] += 1;
+    }
+}
+
 // The int8 rows and their scales for the batched pass (launch_repack_i8): one thread per 8 inputs
 // of a row; the thread of a 32-input block's first 8 writes its scale times 2^k.
 __global__ void k_repack_i8(int8_t *dq, __half *dsc, const int8_t *q, const __half *scales, int rows, int N, int K,
@@ -894,6 +932,50 @@ cudaError_t launch_batch_layer_front(const PrefillDims &d, const PrefillLayer &L
     e = launch_mcol(o, stream, true);
     if (e != cudaSuccess) return e;
     return cudaGetLastError();
+}
+
+cudaError_t launch_pages_layer_front(const PrefillDims &d, const PrefillLayer &L, const PrefillScratch &s, PagesAppend ap,
+                                     PagesAttention at, float *y, float *o, DevState *st, cudaStream_t stream) {
+    const int H = d.hidden, QR = (int)qrows_of(d), A = d.heads * d.head_dim, T = ap.ba.T;
+    const size_t lo = (size_t)d.max_tokens;
+    if (T <= 0 || T > d.max_tokens) return cudaErrorInvalidValue;
+    cudaError_t e = launch_pdl(k_rmsnorm_hilo, T, kNormThreads, stream, s.xa, s.xa + lo * H, s.x, L.in_norm, H, d.eps);
+    if (e != cudaSuccess) return e;
+    McolOp qkv = proj(d, s, L.qkv, MC_STORE, QR, H, s.xa, T, st);
+    qkv.y = y;
+    qkv.ldy = QR;
+    e = launch_mcol(qkv, stream, true);
+    if (e != cudaSuccess) return e;
+    // the packed QKV rows have RoPE partners adjacent; the append takes them apart
+    ap.x = y;
+    ap.x_stride = QR;
+    ap.bias = L.qkv_b;
+    ap.paired = 1;
+    ap.q = s.q;
+    ap.q_stride = A;
+    e = launch_pages_append(ap, stream);
+    if (e != cudaSuccess) return e;
+    at.q = s.q;
+    at.q_stride = A;
+    at.out = o;
+    at.out_stride = A;
+    e = launch_pages_attention(at, stream);
+    if (e != cudaSuccess) return e;
+    const long long n4 = (long long)T * A / 4;
+    e = launch_pdl(k_split_hilo, (unsigned)((n4 + 255) / 256), 256, stream, s.xa, s.xa + lo * A, o, n4);
+    if (e != cudaSuccess) return e;
+    McolOp op = proj(d, s, L.o, MC_RESID, H, A, s.xa, T, st);
+    op.y = s.x;
+    op.ldy = H;
+    return launch_mcol(op, stream, true);
+}
+
+cudaError_t launch_pages_last_rows(float *x_out, const float *x, const PageBatchView &ba, int H, cudaStream_t s) {
+    return launch_pdl(k_pages_last_rows, ba.B, 256, s, x_out, x, ba, H);
+}
+
+cudaError_t launch_pages_advance(int32_t *lens, int32_t *tok, const int32_t *argmax, int32_t *out, int B, cudaStream_t s) {
+    return launch_pdl(k_pages_advance, (B + 127) / 128, 128, s, lens, tok, argmax, out, B);
 }
 
 cudaError_t launch_batch_advance(BatchLane *lanes, int32_t *tok, int32_t *pos, const int32_t *argmax, int32_t *out,

@@ -256,6 +256,43 @@ class CudaQwen2:
                                           C.c_void_p(_stream(self.device))))
         return out
 
+    def new_pages(self, n_pages: int, page_size: int = 64):
+        """Pages for this engine's layers (`paged.PagedKV`: fp16, on its device)."""
+        from .paged import PagedKV
+        return PagedKV(self.cfg.layers, self.cfg.kv_heads, self.cfg.head_dim, n_pages, page_size, torch.float16, self.device)
+
+    def _paged(self, pages, batch, tokens):
+        if pages.layers != self.cfg.layers or pages.device != self.device:
+            raise ValueError(f"pages of {pages.layers} layers on {pages.device} for {self.cfg.layers} on {self.device}")
+        batch._check(pages, 0)
+        if tokens.dtype != torch.int32 or tokens.device != self.device or tokens.numel() < batch.tokens or \
+                not tokens.is_contiguous():
+            raise ValueError(f"tokens: contiguous int32 [{batch.tokens}] on {self.device} expected")
+
+    def forward_pages(self, pages, batch, tokens: torch.Tensor, want_logits: bool = False):
+        """One packed pass of a ragged batch over pages (`sp_forward_pages`): tokens int32 [batch.tokens] on the
+        device, batch.lens counting them. Returns (argmax int32 [B] after each request's last row, logits fp32
+        [B, V] or None)."""
+        self._paged(pages, batch, tokens)
+        argmax = torch.empty(batch.batch, dtype=torch.int32, device=self.device)
+        logits = torch.empty((batch.batch, self.cfg.vocab), dtype=torch.float32, device=self.device) if want_logits else None
+        N.check(N.load().sp_forward_pages(self.handle, pages.layer_array, batch._c, tokens.data_ptr(),
+                                          logits.data_ptr() if want_logits else None, argmax.data_ptr(),
+                                          C.c_void_p(_stream(self.device))))
+        return argmax, logits
+
+    def decode_pages(self, pages, batch, tokens: torch.Tensor, n_steps: int) -> torch.Tensor:
+        """n_steps greedy steps of a batch over pages, fed back on the device (`sp_decode_pages`): tokens int32 [B]
+        holds each request's next token (and its last one afterwards), batch.lens its own keys so far (advanced by
+        n_steps). Returns the argmaxes int32 [n_steps, B]."""
+        self._paged(pages, batch, tokens)
+        if tokens.numel() != batch.batch:
+            raise ValueError(f"tokens: one for each of {batch.batch} requests expected")
+        out = torch.empty((int(n_steps), batch.batch), dtype=torch.int32, device=self.device)
+        N.check(N.load().sp_decode_pages(self.handle, pages.layer_array, batch._c, tokens.data_ptr(), int(n_steps),
+                                         out.data_ptr(), C.c_void_p(_stream(self.device))))
+        return out
+
     def verify_tree(self, kv: DeviceKV, tokens: Sequence[int], parents: Sequence[int], base_pos: int,
                     want_logits: bool = False):
         """One batched pass over a draft tree; returns (argmax int32 [n], logits [n, V] or None)."""

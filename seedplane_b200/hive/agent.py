@@ -42,8 +42,9 @@ class GreedyExecutor:
     Payload: {"ids": [...], "max_new_tokens": n}. Prefill, then the device decode loop (argmax fed
     back on the GPU); one host sync per request, to read the first token. A grouped lease,
     {"batch": [payload, ...]}, runs its requests together (`batch.generate_batch`: one batched pass
-    per decode step for all of them) and answers {"batch": [result, ...]}. Optional `timer`
-    (callable(start: bool)) brackets the device work of each lease."""
+    per decode step for all of them) and answers {"batch": [result, ...]}; with "prefix_ids" beside "batch"
+    every request's ids follow that prefix, which is run and kept once (`batch.generate_shared`). Optional
+    `timer` (callable(start: bool)) brackets the device work of each lease."""
 
     def __init__(self, engine, capacity: int, timer=None):
         self.engine = engine
@@ -52,18 +53,22 @@ class GreedyExecutor:
         self.batch_kvs = []
         self.timer = timer
 
-    def _batch(self, items) -> dict:
-        from ..batch import MAX_BATCH, generate_batch
+    def _batch(self, items, prefix=()) -> dict:
+        from ..batch import MAX_BATCH, generate_batch, generate_shared
         prompts, limits = [], []
         for it in items:
             ids = [int(t) for t in it["ids"]]
             n = int(it.get("max_new_tokens", 32))
             if not ids or n < 1:
                 raise ValueError("a request needs prompt ids and max_new_tokens >= 1")
-            if len(ids) + n > self.capacity:
+            if len(prefix) + len(ids) + n > self.capacity:
                 raise ValueError("request exceeds the agent's KV capacity")
             prompts.append(ids)
             limits.append(n)
+        if prefix:
+            out = generate_shared(self.engine, prefix, prompts, limits, timer=self.timer)
+            dev = str(self.engine.device)
+            return {"batch": [{"tokens": t, "token_sha256": token_sha256(t), "device": dev} for t in out]}
         while len(self.batch_kvs) < min(len(items), MAX_BATCH):
             self.batch_kvs.append(self.engine.new_kv(self.capacity))
         out = []
@@ -76,7 +81,7 @@ class GreedyExecutor:
     def __call__(self, payload: dict) -> dict:
         import torch
         if "batch" in payload:
-            return self._batch(payload["batch"])
+            return self._batch(payload["batch"], [int(t) for t in payload.get("prefix_ids", ())])
         ids = [int(t) for t in payload["ids"]]
         n = int(payload.get("max_new_tokens", 32))
         if not ids or n < 1:

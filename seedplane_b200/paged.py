@@ -8,7 +8,8 @@ attention of a batch reads those once. Three pieces:
 * `PagedKV`: the pages of every layer, [layers][n_pages][kv_heads][page_size][head_dim] for K and for V;
 * `PageBatch`: which rows of a call belong to which request, how many keys each request has, its pages,
   and the prefix all of them start with;
-* `append` and `attention` (`sp_pages_append`, `sp_pages_attention`).
+* `append` and `attention` (`sp_pages_append`, `sp_pages_attention`), which the engine's passes over pages
+  (`CudaQwen2.forward_pages`, `decode_pages`, `batch.generate_shared`) run for every layer.
 
 All of a batch's arrays are device memory that the kernels read, so a CUDA graph captured over them serves
 their later contents. PyTorch only holds memory and streams. The kernels never trap: a bad page number,
@@ -69,6 +70,7 @@ class PagedKV:
                 k_dev=k[i].data_ptr(), v_dev=v[i].data_ptr(), page_stride=k.stride(1), head_stride=k.stride(2),
                 slot_stride=k.stride(3), n_pages=self.n_pages, page_size=self.page_size, kv_heads=self.kv_heads,
                 head_dim=self.head_dim, dtype=_TYPES[k.dtype], status_dev=self._word.data_ptr()))
+        self.layer_array = (N.SpPages * self.layers)(*self._layer)
 
     def status(self):
         """Raise if a kernel met a bad page number, length or position since the last check (waits

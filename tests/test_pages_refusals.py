@@ -97,6 +97,16 @@ def test_bad_chains(lib):
     assert lib.sp_accept_chains_workspace(4, 3, 151936) > 0
 
 
+def test_passes_without_an_engine(lib):
+    one = (N.SpPages * 1)(pages())
+    assert lib.sp_forward_pages(None, one, batch(), PTR, None, PTR, None) == N.SP_ERR_INVALID
+    assert lib.sp_forward_pages(None, None, None, None, None, None, None) == N.SP_ERR_INVALID
+    assert lib.sp_decode_pages(None, one, batch(), PTR, 1, PTR, None) == N.SP_ERR_INVALID
+    assert lib.sp_decode_pages(None, one, batch(), PTR, 0, PTR, None) == N.SP_ERR_INVALID
+    assert lib.sp_decode_pages(None, one, batch(max_q=2, tokens=6), PTR, 1, PTR, None) == N.SP_ERR_INVALID
+    assert lib.sp_decode_pages(None, one, batch(q_start_dev=PTR), PTR, 1, PTR, None) == N.SP_ERR_INVALID
+
+
 def test_python_checks_come_before_the_library():
     from seedplane_b200 import paged, speculative
     k = torch.zeros(4, 2, 16, 64, dtype=torch.float16)
