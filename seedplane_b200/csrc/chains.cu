@@ -2,17 +2,22 @@
 //
 // p_i = softmax(target row i / T), q_i = softmax(draft row i / T); draft i stays while u_i q_i(x_i) <
 // p_i(x_i); the next token is drawn from max(p - q, 0) of the first refused row, or from p_n. Bound by
-// reading the logits once, which is k_chain_stats; what is decided is decided in fp64:
-//   k_chain_stats  (row, chunk): the chunk's maximum, its first index, and the sum of exp((l - max) / T), in
-//                  fp32. In fp64 this pass was bound by the exponentials (159 against 40 us for 352 rows of
-//                  152,064).
-//   k_chain_draw   one cluster of 8 CTAs per request. The rows' sums decide a draft when u q and p differ by more
-//                  than the sums may be off (kChainSlack); otherwise the cluster sums that pair of rows again in
-//                  fp64. The row that is drawn from is summed in fp64 in any case: a draw compares a running
-//                  sum over the vocabulary with a given number, and an fp32 sum of 1e5 terms would move the
-//                  border by more than many tokens' whole probability. An eighth of the vocabulary per CTA (the
-//                  rows mostly still in L2), sums exchanged through distributed shared memory; the CTA that
-//                  holds the drawn number finds its index.
+// reading the logits once, which is k_chain_stats; what is decided is decided in fp64, on the one or two rows a
+// request draws from (mostly still in L2):
+//   k_chain_stats   (row, chunk): the chunk's maximum, its first index, and the sum of exp((l - max) / T), in
+//                   fp32. In fp64 this pass was bound by the exponentials (159 against 41 us for 352 rows of
+//                   152,064).
+//   k_chain_decide  a CTA per request: joins the chunks and walks the chain. The rows' sums decide a draft when u q
+//                   and p differ by more than the sums may be off (kChainSlack); a draft that is nearer (one in
+//                   10,000) leaves the request to the slow walk in k_chain_pick.
+//   k_chain_sums    (request, piece of the vocabulary): fp64 sums of the rows that are drawn from. A draw compares a
+//                   running sum over the vocabulary with a given number, and an fp32 sum of 1e5 terms would move the
+//                   border by more than many tokens' whole probability.
+//   k_chain_left    (request, piece): fp64 sums of max(p - q, 0), for requests with a refused draft and a drafter
+//   k_chain_pick    a CTA per request: the piece and in it the index whose running sum passes u times the total
+// The pieces spread the requests' fp64 work (four exponentials a token after a refusal, else one) over all SMs; a
+// cluster of 8 CTAs per request for the last four took 43 us for 32 requests and 36 for 48 without a drafter, these
+// 40 and 24.
 // How far k_chain_stats' sum may be off, relatively: z = (l - max) / T in base 2 carries two roundings and 1 / T a
 // third (3 2^-24 |z|, and terms below 2^-60 of the largest weigh nothing: 2^-16.5 at |z| = 60), the
 // exponential 2^-22, the sums over a thread's 32 terms, a warp, a CTA and the chunks at most 60 2^-24: below
@@ -31,10 +36,10 @@ namespace {
 constexpr int kStatThreads = 256;
 constexpr int kStatChunk = 8192;             // logits per CTA of k_chain_stats
 constexpr int kStatPer = kStatChunk / kStatThreads;
-constexpr int kDrawCtas = 8;                 // CTAs (a cluster) per request
-constexpr int kDrawThreads = 512;
-constexpr int kDrawWarps = kDrawThreads / 32;
-constexpr int kBatch = 8;                    // logits a thread of k_chain_draw has under way
+constexpr int kPieceThreads = 256;
+constexpr int kPiece = 4096;                 // logits per CTA of k_chain_sums and k_chain_left
+constexpr int kBatch = 8;                    // logits a thread has under way
+constexpr int kPickThreads = 512;
 constexpr double kChainSlack = 1.0 / 16384;  // 2^-14: four times two sums' bound
 
 struct ChainStat {                           // of a chunk or a row
@@ -180,287 +185,428 @@ struct Weigh {                               // exp((l - max) / T) of a row's lo
     }
 };
 
-SP_DEVINL void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+// ---- the draw ----------------------------------------------------------------------------------
+enum ChainMode : int { CM_DONE = 0, CM_P = 1, CM_P_LESS = 2, CM_BOTH = 3, CM_SLOW = 4 };
+struct ChainPlan {                           // of a request, by k_chain_decide
+    int mode;                                // weights: none (the token is written), p, p without the refused token,
+                                             // max(p - q, 0); or the slow walk
+    int acc;                                 // accepted drafts: the row that is drawn from
+    float mp, mq;                            // the rows' maxima
+};
+struct ChainScratch {
+    ChainStat *st;                           // [B][rows][chunks]
+    ChainPlan *plan;                         // [B]
+    double *sp, *sq, *left;                  // [B][pieces]
+};
+__host__ __device__ inline int chain_pieces(int V) { return (V + kPiece - 1) / kPiece; }
+
+SP_DEVINL Weigh chain_weigh(const ChainArgs &a, int b, double *tab) {
+    if (threadIdx.x < 64) tab[threadIdx.x] = c_exp_tab[threadIdx.x];
+    return Weigh{tab, chain_inv_t(a, b) * 92.33248261689365807103517958412109, chain_k2(a, b)};
 }
-SP_DEVINL double ld_peer(const double *p, uint32_t rank) {
-    uint32_t at;
-    double v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(at) : "memory");
-    return v;
+// sums of a CTA, the same bits in every thread
+template <int THREADS>
+SP_DEVINL void cta_sums(double &x, double &y, double (*s_sum)[THREADS / 32]) {
+    for (int o = 16; o > 0; o >>= 1) {
+        x += __shfl_xor_sync(0xffffffffu, x, o);
+        y += __shfl_xor_sync(0xffffffffu, y, o);
+    }
+    __syncthreads();                                         // s_sum of the time before is read
+    if ((threadIdx.x & 31) == 0) {
+        s_sum[0][threadIdx.x >> 5] = x;
+        s_sum[1][threadIdx.x >> 5] = y;
+    }
+    __syncthreads();
+    x = y = 0.0;
+    for (int w = 0; w < THREADS / 32; ++w) {
+        x += s_sum[0][w];
+        y += s_sum[1][w];
+    }
 }
 
+constexpr int kDecideThreads = 256;
 template <typename T>
-__global__ void __cluster_dims__(kDrawCtas, 1, 1) __launch_bounds__(kDrawThreads) k_chain_draw(ChainArgs a, const ChainStat *st) {
+__global__ void __launch_bounds__(kDecideThreads) k_chain_decide(ChainArgs a, ChainScratch sc) {
     __shared__ ChainStat s_row[2 * kChainMaxDrafts + 1];
-    __shared__ double s_tab[64], s_warp[2][kDrawWarps], s_ex[2][2], s_all[2][kDrawCtas];
-    __shared__ int s_dec[kChainMaxDrafts], s_pick, s_last;
-    const int b = blockIdx.x / kDrawCtas, rank = blockIdx.x - b * kDrawCtas;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    __shared__ double s_tab[64];
+    __shared__ int s_dec[kChainMaxDrafts];
+    griddep_launch_dependents();
+    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rows = chain_rows(a), chunks = chain_chunks(a.V), cnt = chain_count(a, b);
     const double inv_t = chain_inv_t(a, b);
     const float k2 = chain_k2(a, b);
-    const Weigh weigh{s_tab, inv_t * 92.33248261689365807103517958412109, k2};
+    const Weigh weigh = chain_weigh(a, b, s_tab);
     const int *tokens = a.tokens + (size_t)b * a.n;
-    const double *u = a.u + (size_t)b * (a.n + 1);
-    if (tid < 64) s_tab[tid] = c_exp_tab[tid];
-    if (tid == 0) {
-        s_pick = INT_MAX;
-        s_last = -1;
+    // thread i decides draft i: its token, and the token's logits, do not wait for the statistics
+    int x = -1;
+    float lp = -INFINITY, lq = -INFINITY;
+    double u = 0.0;
+    if (tid < cnt) {
+        x = tokens[tid];
+        u = a.u[(size_t)b * (a.n + 1) + tid];
+        if (x >= 0 && x < a.V) {
+            lp = to_float(chain_row<T>(a, b, tid)[x]);
+            if (a.draft) lq = to_float(chain_row<T>(a, b, a.n + 1 + tid)[x]);
+        }
     }
     griddep_wait();
     // the rows' statistics: a warp per row, lanes over the chunks
-    for (int r = warp; r < rows; r += kDrawWarps) {
-        ChainStat x{0.f, -INFINITY, INT_MAX, 0};
+    for (int r = warp; r < rows; r += kDecideThreads / 32) {
+        ChainStat s{0.f, -INFINITY, INT_MAX, 0};
         if (r <= a.n ? r <= cnt : r - a.n - 1 < cnt) {
-            const ChainStat *c = st + ((size_t)b * rows + r) * chunks;
-            for (int k = lane; k < chunks; k += 32) stat_join(x, c[k], k2);
+            const ChainStat *c = sc.st + ((size_t)b * rows + r) * chunks;
+            for (int k = lane; k < chunks; k += 32) stat_join(s, c[k], k2);
             for (int o = 16; o > 0; o >>= 1) {
-                ChainStat y{__shfl_xor_sync(0xffffffffu, x.sum, o), __shfl_xor_sync(0xffffffffu, x.max, o),
-                            __shfl_xor_sync(0xffffffffu, x.first, o), 0};
-                stat_join(x, y, k2);
+                ChainStat y{__shfl_xor_sync(0xffffffffu, s.sum, o), __shfl_xor_sync(0xffffffffu, s.max, o),
+                            __shfl_xor_sync(0xffffffffu, s.first, o), 0};
+                stat_join(s, y, k2);
             }
         }
-        if (lane == 0) s_row[r] = x;
+        if (lane == 0) s_row[r] = s;
     }
     __syncthreads();
-    // thread i decides draft i: 0 refused, 1 accepted, 2 too near to say
-    if (tid < cnt) {
-        const int x = tokens[tid];
+    if (tid < cnt) {                                         // 0 refused, 1 accepted, 2 too near to say
         const ChainStat tp = s_row[tid];
         int dec = 0;
         if (x >= 0 && x < a.V && tp.max > -INFINITY) {
             if (inv_t == 0.0) {
                 dec = x == tp.first;
             } else {
-                const double px = weigh(to_float(chain_row<T>(a, b, tid)[x]), tp.max) / tp.sum;
+                const double px = weigh(lp, tp.max) / tp.sum;
                 double qx = 1.0;
                 if (a.draft) {
                     const ChainStat dq = s_row[a.n + 1 + tid];
-                    qx = dq.max > -INFINITY ? weigh(to_float(chain_row<T>(a, b, a.n + 1 + tid)[x]), dq.max) / dq.sum : 0.0;
+                    qx = dq.max > -INFINITY ? weigh(lq, dq.max) / dq.sum : 0.0;
                 }
-                const double uq = u[tid] * qx;
+                const double uq = u * qx;
                 dec = px == 0.0 ? 0 : fabs(uq - px) <= kChainSlack * px ? 2 : uq < px;
             }
         }
         s_dec[tid] = dec;
     }
     __syncthreads();
-
-    // this CTA's slice of the vocabulary, a contiguous piece of it per warp
-    const int slice = (a.V + kDrawCtas - 1) / kDrawCtas, piece = (slice + kDrawWarps - 1) / kDrawWarps;
-    const int s_lo = min(a.V, rank * slice), s_hi = min(a.V, s_lo + slice);
-    const int w_lo = min(s_hi, s_lo + warp * piece), w_hi = min(s_hi, w_lo + piece);
-    int round = 0;
-    // two sums over the cluster, the same bits in every thread: each warp's x, y -> the CTAs' in s_all, the
-    // totals in x, y
-    const auto exchange = [&](double &x, double &y) {
-        for (int o = 16; o > 0; o >>= 1) {
-            x += __shfl_xor_sync(0xffffffffu, x, o);
-            y += __shfl_xor_sync(0xffffffffu, y, o);
-        }
-        __syncthreads();                                     // s_warp and s_all of the round before are read
-        if (lane == 0) {
-            s_warp[0][warp] = x;
-            s_warp[1][warp] = y;
-        }
-        __syncthreads();
-        if (tid < 2) {
-            double sum = 0.0;
-            for (int w = 0; w < kDrawWarps; ++w) sum += s_warp[tid][w];
-            s_ex[round & 1][tid] = sum;                      // a peer reads it before the barrier after next
-        }
-        cluster_barrier();
-        if (tid < 2 * kDrawCtas) s_all[tid & 1][tid >> 1] = ld_peer(&s_ex[round & 1][tid & 1], tid >> 1);
-        __syncthreads();
-        ++round;
-        x = y = 0.0;
-        for (int c = 0; c < kDrawCtas; ++c) {
-            x += s_all[0][c];
-            y += s_all[1][c];
-        }
-    };
-    // the sums of target row i and, with a drafter, draft row i
-    const auto pair_sums = [&](int i, bool both, double &sp, double &sq) {
-        const T *pr = chain_row<T>(a, b, i), *qr = both ? chain_row<T>(a, b, a.n + 1 + i) : pr;
-        const float mp = s_row[i].max, mq = both ? s_row[a.n + 1 + i].max : 0.f;
-        sp = sq = 0.0;
-        for (int j0 = w_lo + lane; j0 < w_hi; j0 += 32 * kBatch) {
-            float x[kBatch], y[kBatch];
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                const int j = j0 + 32 * i;
-                x[i] = j < w_hi ? to_float(pr[j]) : -INFINITY;
-                y[i] = both && j < w_hi ? to_float(qr[j]) : -INFINITY;
-            }
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i) sp += weigh(x[i], mp);
-            if (both) {
-#pragma unroll
-                for (int i = 0; i < kBatch; ++i) sq += weigh(y[i], mq);
-            }
-        }
-        exchange(sp, sq);
-    };
-
     int acc = 0;
-    double sp = 0.0, sq = 0.0;
-    bool summed = false;                                     // sp, sq are those of row acc
-    for (; acc < cnt; ++acc) {                               // the same walk in every thread of the cluster
-        int dec = s_dec[acc];
-        summed = false;
-        if (dec == 2) {
-            const bool both = a.draft && s_row[a.n + 1 + acc].max > -INFINITY;
-            pair_sums(acc, both, sp, sq);
-            summed = true;
-            const int x = tokens[acc];
-            const double px = weigh(to_float(chain_row<T>(a, b, acc)[x]), s_row[acc].max) / sp;
-            const double qx = both ? weigh(to_float(chain_row<T>(a, b, a.n + 1 + acc)[x]), s_row[a.n + 1 + acc].max) / sq
-                                   : a.draft ? 0.0 : 1.0;
-            dec = u[acc] * qx < px;
-        }
-        if (dec == 0) break;
-    }
-    const ChainStat tp = s_row[acc];
+    while (acc < cnt && s_dec[acc] == 1) ++acc;
+    const bool refused = acc < cnt;
+    ChainPlan plan{CM_DONE, acc, s_row[acc].max, refused && a.draft ? s_row[a.n + 1 + acc].max : -INFINITY};
     int pick = -1;
-    bool write = rank == 0;                                  // of the drawn token
-    if (inv_t == 0.0) {
-        if (tp.max > -INFINITY) pick = tp.first;
-    } else if (tp.max > -INFINITY) {
-        write = false;
-        // the weights: max(p - q, 0), or p (all accepted; or nothing left of p - q)
-        const bool refused = acc < cnt;
-        const T *pr = chain_row<T>(a, b, acc);
-        const int x = refused ? tokens[acc] : -1;
-        const bool both = refused && a.draft && s_row[a.n + 1 + acc].max > -INFINITY;
-        const T *qr = both ? chain_row<T>(a, b, a.n + 1 + acc) : nullptr;
-        const float mq = both ? s_row[a.n + 1 + acc].max : 0.f;
-        // without a drafter's row the weights are p's, less the refused token: no sum to divide by
-        if (both && !summed) pair_sums(acc, true, sp, sq);
-        const double ip = both ? 1.0 / sp : 0.0, iq = both ? 1.0 / sq : 0.0;
-        bool residual = refused && (both || !a.draft);       // a drafter's row that weighs nothing takes nothing away
-        // both products rounded (no fused multiply-add): equal rows leave exactly nothing
-        const auto left = [&](int j) -> double {
-            if (both && residual)
-                return fmax(__dmul_rn(weigh(to_float(pr[j]), tp.max), ip) - __dmul_rn(weigh(to_float(qr[j]), mq), iq), 0.0);
-            return residual && j == x ? 0.0 : weigh(to_float(pr[j]), tp.max);    // p(x) - 1 is not positive
-        };
-        double total;
-        for (;;) {
-            double none = 0.0;
-            total = 0.0;
-            for (int j0 = w_lo + lane; j0 < w_hi; j0 += 32 * kBatch) {
-                float lp[kBatch], lq[kBatch];
-#pragma unroll
-                for (int i = 0; i < kBatch; ++i) {
-                    const int j = j0 + 32 * i;
-                    lp[i] = j < w_hi ? to_float(pr[j]) : -INFINITY;
-                    lq[i] = both && residual && j < w_hi ? to_float(qr[j]) : -INFINITY;
-                }
-                if (both && residual) {
-#pragma unroll
-                    for (int i = 0; i < kBatch; ++i)
-                        total += fmax(__dmul_rn(weigh(lp[i], tp.max), ip) - __dmul_rn(weigh(lq[i], mq), iq), 0.0);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < kBatch; ++i)
-                        total += weigh(residual && j0 + 32 * i == x ? -INFINITY : lp[i], tp.max);
-                }
-            }
-            exchange(total, none);
-            if (total > 0.0 || !residual) break;
-            residual = false;                                // nothing left of p - q: p itself
-        }
-        // the first CTA, warp and index whose running sum passes `want`; where rounding lets none of them
-        // pass it, the last one that weighs anything
-        const double want = u[a.n] * total;
-        double run = 0.0, before = 0.0;
-        int owner = -1;
-        for (int c = 0; c < kDrawCtas; ++c) {
-            const double next = run + s_all[0][c];
-            if (s_all[0][c] > 0.0) {
-                owner = c;
-                before = run;
-                if (next > want) break;
-            }
-            run = next;
-        }
-        if (owner == rank) {
-            int w_own = 0;
-            double base = before;
-            run = before;
-            for (int w = 0; w < kDrawWarps; ++w) {
-                const double next = run + s_warp[0][w];
-                if (s_warp[0][w] > 0.0) {
-                    w_own = w;
-                    base = run;
-                    if (next > want) break;
-                }
-                run = next;
-            }
-            // that warp's piece again, a few indices a thread
-            const int p_lo = min(s_hi, s_lo + w_own * piece), p_hi = min(s_hi, p_lo + piece);
-            const int per = (p_hi - p_lo + kDrawThreads - 1) / kDrawThreads;
-            const int t_lo = min(p_hi, p_lo + tid * per), t_hi = min(p_hi, t_lo + per);
-            double mine = 0.0;
-            int last = -1;
-            for (int j = t_lo; j < t_hi; ++j) {
-                const double w = left(j);
-                mine += w;
-                if (w > 0.0) last = j;
-            }
-            double incl = mine;
-            for (int o = 1; o < 32; o <<= 1) {
-                const double y = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += y;
-            }
-            __syncthreads();                                 // s_warp is read
-            if (lane == 31) s_warp[0][warp] = incl;
-            __syncthreads();
-            run = base;
-            for (int w = 0; w < warp; ++w) run += s_warp[0][w];
-            const double from_here = run + incl - mine;
-            if (mine > 0.0) {
-                run = from_here;
-                for (int j = t_lo; j < t_hi; ++j) {
-                    const double w = left(j);
-                    run += w;
-                    if (w > 0.0 && run > want) {
-                        atomicMin(&s_pick, j);
-                        break;
-                    }
-                }
-                atomicMax(&s_last, last);
-            }
-            __syncthreads();
-            pick = s_pick != INT_MAX ? s_pick : s_last;
-            write = true;
-        }
-    }
-    // write: rank 0 the accepted tokens and the tail, the CTA that found it the drawn one
-    int *out = a.out_tokens + (size_t)b * (a.n + 1);
-    if (rank == 0) {
-        for (int i = tid; i <= a.n; i += kDrawThreads)
+    if (refused && s_dec[acc] == 2) plan.mode = CM_SLOW;
+    else if (plan.mp == -INFINITY) pick = -1;
+    else if (inv_t == 0.0) pick = s_row[acc].first;
+    else if (!refused || (a.draft && plan.mq == -INFINITY)) plan.mode = CM_P;    // a drafter's empty row takes nothing away
+    else plan.mode = a.draft ? CM_BOTH : CM_P_LESS;
+    if (tid == 0) sc.plan[b] = plan;
+    if (plan.mode != CM_SLOW) {
+        int *out = a.out_tokens + (size_t)b * (a.n + 1);
+        for (int i = tid; i <= a.n; i += kDecideThreads)
             if (i != acc) out[i] = i < acc ? tokens[i] : -1;
+            else if (plan.mode == CM_DONE) out[i] = pick;
         if (tid == 0) a.accepted[b] = acc;
     }
-    if (write && tid == 0) out[acc] = pick;
-    cluster_barrier();                                       // no CTA ends while a peer reads its sums
+}
+
+// f(index, logits) of a piece [lo, hi) of row pr and, if given, qr
+template <typename T, int THREADS, typename F>
+SP_DEVINL void walk_piece(const T *pr, const T *qr, int lo, int hi, F f) {
+    for (int j0 = lo + threadIdx.x; j0 < hi; j0 += THREADS * kBatch) {
+        float x[kBatch], y[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int j = j0 + THREADS * i;
+            x[i] = j < hi ? to_float(pr[j]) : -INFINITY;
+            y[i] = qr && j < hi ? to_float(qr[j]) : -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) f(j0 + THREADS * i, x[i], y[i]);
+    }
+}
+// max(p - q, 0) of a token; both products rounded (no fused multiply-add): equal rows leave exactly nothing
+SP_DEVINL double left_of(double ep, double ip, double eq, double iq) {
+    return fmax(__dmul_rn(ep, ip) - __dmul_rn(eq, iq), 0.0);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPieceThreads) k_chain_sums(ChainArgs a, ChainScratch sc) {
+    __shared__ double s_tab[64], s_sum[2][kPieceThreads / 32];
+    griddep_launch_dependents();
+    const int pieces = chain_pieces(a.V), b = blockIdx.x / pieces, k = blockIdx.x - b * pieces;
+    const Weigh weigh = chain_weigh(a, b, s_tab);
+    __syncthreads();
+    griddep_wait();
+    const ChainPlan plan = sc.plan[b];
+    if (plan.mode == CM_DONE || plan.mode == CM_SLOW) return;
+    const int lo = k * kPiece, hi = min(a.V, lo + kPiece);
+    const T *pr = chain_row<T>(a, b, plan.acc);
+    double sp = 0.0, sq = 0.0;
+    if (plan.mode == CM_BOTH) {
+        walk_piece<T, kPieceThreads>(pr, chain_row<T>(a, b, a.n + 1 + plan.acc), lo, hi, [&](int, float x, float y) {
+            sp += weigh(x, plan.mp);
+            sq += weigh(y, plan.mq);
+        });
+    } else {
+        const int out = plan.mode == CM_P_LESS ? a.tokens[(size_t)b * a.n + plan.acc] : -1;    // p(x) - 1 is not positive
+        walk_piece<T, kPieceThreads>(pr, (const T *)nullptr, lo, hi, [&](int j, float x, float) {
+            sp += weigh(j == out ? -INFINITY : x, plan.mp);
+        });
+    }
+    cta_sums<kPieceThreads>(sp, sq, s_sum);
+    if (threadIdx.x == 0) {
+        sc.sp[blockIdx.x] = sp;
+        sc.sq[blockIdx.x] = sq;
+    }
+}
+
+// a request's totals of two piece arrays: the same tree, and so the same bits, in every warp of every kernel
+SP_DEVINL void piece_totals(const double *x, const double *y, int pieces, double &sx, double &sy) {
+    sx = sy = 0.0;
+    for (int k = threadIdx.x & 31; k < pieces; k += 32) {
+        sx += x[k];
+        sy += y[k];
+    }
+    for (int o = 16; o > 0; o >>= 1) {
+        sx += __shfl_xor_sync(0xffffffffu, sx, o);
+        sy += __shfl_xor_sync(0xffffffffu, sy, o);
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPieceThreads) k_chain_left(ChainArgs a, ChainScratch sc) {
+    __shared__ double s_tab[64], s_sum[2][kPieceThreads / 32];
+    griddep_launch_dependents();
+    const int pieces = chain_pieces(a.V), b = blockIdx.x / pieces, k = blockIdx.x - b * pieces;
+    const Weigh weigh = chain_weigh(a, b, s_tab);
+    __syncthreads();
+    griddep_wait();
+    const ChainPlan plan = sc.plan[b];
+    if (plan.mode != CM_BOTH) return;
+    double sp, sq;
+    piece_totals(sc.sp + (size_t)b * pieces, sc.sq + (size_t)b * pieces, pieces, sp, sq);
+    const double ip = 1.0 / sp, iq = 1.0 / sq;
+    const int lo = k * kPiece, hi = min(a.V, lo + kPiece);
+    double sum = 0.0, none = 0.0;
+    walk_piece<T, kPieceThreads>(chain_row<T>(a, b, plan.acc), chain_row<T>(a, b, a.n + 1 + plan.acc), lo, hi,
+                                 [&](int, float x, float y) { sum += left_of(weigh(x, plan.mp), ip, weigh(y, plan.mq), iq); });
+    cta_sums<kPieceThreads>(sum, none, s_sum);
+    if (threadIdx.x == 0) sc.left[blockIdx.x] = sum;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPickThreads) k_chain_pick(ChainArgs a, ChainScratch sc) {
+    __shared__ double s_tab[64], s_sum[2][kPickThreads / 32];
+    __shared__ int s_pick, s_last;
+    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int pieces = chain_pieces(a.V);
+    const Weigh weigh = chain_weigh(a, b, s_tab);
+    const double *u = a.u + (size_t)b * (a.n + 1);
+    const int *tokens = a.tokens + (size_t)b * a.n;
+    if (tid == 0) {
+        s_pick = INT_MAX;
+        s_last = -1;
+    }
+    __syncthreads();
+    griddep_wait();
+    ChainPlan plan = sc.plan[b];
+    if (plan.mode == CM_DONE) return;
+    double *sp = sc.sp + (size_t)b * pieces, *sq = sc.sq + (size_t)b * pieces, *left = sc.left + (size_t)b * pieces;
+    const auto maximum = [&](const T *row) {                 // NaN ignored, the same in every thread
+        float m = -INFINITY;
+        for (int j = tid; j < a.V; j += kPickThreads) m = fmaxf(m, to_float(row[j]));
+        double d = warp_max(m);
+        __syncthreads();
+        if (lane == 0) s_sum[0][warp] = d;
+        __syncthreads();
+        d = s_sum[0][0];
+        for (int w = 1; w < kPickThreads / 32; ++w) d = fmax(d, s_sum[0][w]);
+        return (float)d;
+    };
+    // the pieces' sums by this CTA alone: fp(logit p), fq(logit q) into sp, sq, or one function into left
+    const auto sums_here = [&](const T *pr, const T *qr, bool residual, double ip, double iq, double &tx, double &ty) {
+        tx = ty = 0.0;
+        for (int k = 0; k < pieces; ++k) {
+            double x = 0.0, y = 0.0;
+            walk_piece<T, kPickThreads>(pr, qr, k * kPiece, min(a.V, (k + 1) * kPiece), [&](int, float lp, float lq) {
+                const double ep = weigh(lp, plan.mp), eq = weigh(lq, plan.mq);
+                if (residual) {
+                    x += left_of(ep, ip, eq, iq);
+                } else {
+                    x += ep;
+                    y += eq;
+                }
+            });
+            cta_sums<kPickThreads>(x, y, s_sum);
+            if (tid == 0) {
+                (residual ? left : sp)[k] = x;
+                if (!residual) sq[k] = y;
+            }
+            tx += x;
+            ty += y;
+        }
+        __syncthreads();
+    };
+    if (plan.mode == CM_SLOW) {
+        // the walk on from the draft that was too near, every decision from fp64 sums
+        const int cnt = chain_count(a, b);
+        double tp = 0.0, tq = 0.0;
+        for (;; ++plan.acc) {
+            const bool last = plan.acc >= cnt;
+            const T *pr = chain_row<T>(a, b, plan.acc), *qr = !last && a.draft ? chain_row<T>(a, b, a.n + 1 + plan.acc) : nullptr;
+            plan.mp = maximum(pr);
+            plan.mq = qr ? maximum(qr) : -INFINITY;
+            plan.mode = CM_DONE;
+            if (plan.mp == -INFINITY) break;
+            sums_here(pr, qr, false, 0.0, 0.0, tp, tq);
+            plan.mode = CM_P;
+            if (last) break;
+            const int x = tokens[plan.acc];
+            const bool in = x >= 0 && x < a.V;
+            const double px = in ? weigh(to_float(pr[x]), plan.mp) / tp : 0.0;
+            const double qx = !a.draft ? 1.0 : plan.mq > -INFINITY && in ? weigh(to_float(qr[x]), plan.mq) / tq : 0.0;
+            if (in && u[plan.acc] * qx < px) continue;
+            if (a.draft && plan.mq > -INFINITY) {
+                plan.mode = CM_BOTH;
+                double none;
+                sums_here(pr, qr, true, 1.0 / tp, 1.0 / tq, tq, none);
+            } else if (!a.draft) {
+                plan.mode = CM_P_LESS;
+                if (in && tid == 0) {                        // the refused token out of its piece
+                    double y = 0.0;
+                    const int k = x / kPiece;
+                    for (int j = k * kPiece; j < min(a.V, (k + 1) * kPiece); ++j)
+                        if (j != x) y += weigh(to_float(pr[j]), plan.mp);
+                    sp[k] = y;
+                }
+                __syncthreads();
+            }
+            break;
+        }
+        int *out = a.out_tokens + (size_t)b * (a.n + 1);
+        for (int i = tid; i <= a.n; i += kPickThreads) out[i] = i < plan.acc ? tokens[i] : -1;
+        if (tid == 0) a.accepted[b] = plan.acc;
+        __syncthreads();
+        if (plan.mode == CM_DONE) return;
+    }
+    const T *pr = chain_row<T>(a, b, plan.acc), *qr = plan.mode == CM_BOTH ? chain_row<T>(a, b, a.n + 1 + plan.acc) : nullptr;
+    double tp, tq, total, ip = 0.0, iq = 0.0;
+    piece_totals(sp, sq, pieces, tp, tq);
+    const double *weights = sp;
+    total = tp;
+    int without = plan.mode == CM_P_LESS ? tokens[plan.acc] : -1;
+    if (plan.mode == CM_BOTH) {
+        double none;
+        piece_totals(left, left, pieces, total, none);
+        if (total > 0.0) {
+            weights = left;
+            ip = 1.0 / tp;
+            iq = 1.0 / tq;
+        } else {                                             // nothing left of p - q: p itself
+            qr = nullptr;
+            total = tp;
+        }
+    } else if (plan.mode == CM_P_LESS && !(total > 0.0)) {   // p is 1 at the refused token
+        if (tid == 0) a.out_tokens[(size_t)b * (a.n + 1) + plan.acc] = without;
+        return;
+    }
+    // the first piece and index whose running sum passes `want`; where rounding lets none of them pass it, the
+    // last one that weighs anything
+    const double want = u[a.n] * total;
+    double run = 0.0, base = 0.0;
+    int own = 0;
+    for (int k0 = 0; k0 < pieces; k0 += 32) {                // 32 pieces at a time, every warp alike
+        const double w = k0 + lane < pieces ? weights[k0 + lane] : 0.0;
+        double incl = w;
+        for (int o = 1; o < 32; o <<= 1) {
+            const double y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        const unsigned some = __ballot_sync(0xffffffffu, w > 0.0);
+        const unsigned over = __ballot_sync(0xffffffffu, w > 0.0 && run + incl > want);
+        if (some) {
+            const int at = over ? __ffs(over) - 1 : 31 - __clz(some);
+            own = k0 + at;
+            base = run + __shfl_sync(0xffffffffu, incl - w, at);
+            if (over) break;
+        }
+        run += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    const int lo = own * kPiece, hi = min(a.V, lo + kPiece);
+    constexpr int PER = kPiece / kPickThreads;               // consecutive indices of a thread
+    double w[PER], mine = 0.0;
+    int last = -1;
+    float lp[PER], lq[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int j = lo + tid * PER + i;
+        lp[i] = j < hi && j != without ? to_float(pr[j]) : -INFINITY;
+        lq[i] = qr && j < hi ? to_float(qr[j]) : -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const double ep = weigh(lp[i], plan.mp);
+        w[i] = qr ? left_of(ep, ip, weigh(lq[i], plan.mq), iq) : ep;
+        mine += w[i];
+        if (w[i] > 0.0) last = lo + tid * PER + i;
+    }
+    double incl = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+    }
+    if (lane == 31) s_sum[0][warp] = incl;
+    __syncthreads();
+    run = base;
+    for (int k = 0; k < warp; ++k) run += s_sum[0][k];
+    run += incl - mine;
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        run += w[i];
+        if (!found && w[i] > 0.0 && run > want) {
+            found = true;
+            atomicMin(&s_pick, lo + tid * PER + i);
+        }
+    }
+    if (last >= 0) atomicMax(&s_last, last);
+    __syncthreads();
+    if (tid == 0) a.out_tokens[(size_t)b * (a.n + 1) + plan.acc] = s_pick != INT_MAX ? s_pick : s_last;
+}
+
+size_t up16(size_t v) { return (v + 15) / 16 * 16; }
+ChainScratch chain_scratch(const ChainArgs &a, void *base) {
+    uint8_t *p = static_cast<uint8_t *>(base);
+    const auto take = [&](size_t bytes) { uint8_t *q = p; p += up16(bytes); return q; };
+    const size_t pieces = (size_t)a.B * chain_pieces(a.V) * sizeof(double);
+    ChainScratch sc{};
+    sc.st = reinterpret_cast<ChainStat *>(take((size_t)a.B * (2 * a.n + 1) * chain_chunks(a.V) * sizeof(ChainStat)));
+    sc.plan = reinterpret_cast<ChainPlan *>(take((size_t)a.B * sizeof(ChainPlan)));
+    sc.sp = reinterpret_cast<double *>(take(pieces));
+    sc.sq = reinterpret_cast<double *>(take(pieces));
+    sc.left = reinterpret_cast<double *>(take(pieces));
+    return sc;
 }
 
 template <typename T>
 cudaError_t chains_typed(const ChainArgs &a, cudaStream_t s) {
-    ChainStat *st = static_cast<ChainStat *>(a.ws);
-    k_chain_stats<T><<<(unsigned)(a.B * chain_rows(a) * chain_chunks(a.V)), kStatThreads, 0, s>>>(a, st);
+    const ChainScratch sc = chain_scratch(a, a.ws);
+    k_chain_stats<T><<<(unsigned)(a.B * chain_rows(a) * chain_chunks(a.V)), kStatThreads, 0, s>>>(a, sc.st);
     cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-    return launch_dependent(k_chain_draw<T>, dim3(a.B * kDrawCtas), kDrawThreads, 0, s, a, st);
+    const dim3 pieces((unsigned)(a.B * chain_pieces(a.V)));
+    if (e == cudaSuccess) e = launch_dependent(k_chain_decide<T>, dim3(a.B), kDecideThreads, 0, s, a, sc);
+    if (e == cudaSuccess) e = launch_dependent(k_chain_sums<T>, pieces, kPieceThreads, 0, s, a, sc);
+    if (e == cudaSuccess && a.draft) e = launch_dependent(k_chain_left<T>, pieces, kPieceThreads, 0, s, a, sc);
+    if (e == cudaSuccess) e = launch_dependent(k_chain_pick<T>, dim3(a.B), kPickThreads, 0, s, a, sc);
+    return e;
 }
 
 }  // namespace
 
-size_t chains_workspace(int B, int n, int V) { return (size_t)B * (2 * n + 1) * chain_chunks(V) * sizeof(ChainStat); }
+size_t chains_workspace(int B, int n, int V) {
+    ChainArgs a{};
+    a.B = B;
+    a.n = n;
+    a.V = V;
+    const ChainScratch sc = chain_scratch(a, nullptr);
+    return reinterpret_cast<size_t>(sc.left) + up16((size_t)B * chain_pieces(V) * sizeof(double));
+}
 
 cudaError_t launch_accept_chains(const ChainArgs &a, cudaStream_t s) {
     if (a.type == VT_F32) return chains_typed<float>(a, s);
