@@ -7,12 +7,12 @@
 //   k_chain_stats   (row, chunk): the chunk's maximum, its first index, and the sum of exp((l - max) / T), in
 //                   fp32. In fp64 this pass was bound by the exponentials (159 against 41 us for 352 rows of
 //                   152,064).
-//   k_chain_decide  a CTA per request: joins the chunks and walks the chain. The rows' sums decide a draft when u q
-//                   and p differ by more than the sums may be off (kChainSlack); a draft that is nearer (one in
-//                   10,000) leaves the request to the slow walk in k_chain_pick.
-//   k_chain_sums    (request, piece of the vocabulary): fp64 sums of the rows that are drawn from. A draw compares a
-//                   running sum over the vocabulary with a given number, and an fp32 sum of 1e5 terms would move the
-//                   border by more than many tokens' whole probability.
+//   k_chain_sums    (request, piece of the vocabulary): joins the chunks and walks the chain (every piece's CTA for
+//                   itself: less than a launch), then fp64 sums of the rows that are drawn from. The rows' fp32
+//                   sums decide a draft when u q and p differ by more than the sums may be off (kChainSlack); a
+//                   draft that is nearer (one in 10,000) leaves the request to the slow walk in k_chain_pick. A draw
+//                   compares a running sum over the vocabulary with a given number, and an fp32 sum of 1e5 terms
+//                   would move the border by more than many tokens' whole probability.
 //   k_chain_left    (request, piece): fp64 sums of max(p - q, 0), for requests with a refused draft and a drafter
 //   k_chain_pick    a CTA per request: the piece and in it the index whose running sum passes u times the total
 // The pieces spread the requests' fp64 work (four exponentials a token after a refusal, else one) over all SMs; a
@@ -37,7 +37,7 @@ constexpr int kStatThreads = 256;
 constexpr int kStatChunk = 8192;             // logits per CTA of k_chain_stats
 constexpr int kStatPer = kStatChunk / kStatThreads;
 constexpr int kPieceThreads = 256;
-constexpr int kPiece = 4096;                 // logits per CTA of k_chain_sums and k_chain_left
+constexpr int kPieceMost = 4096;             // logits per CTA of k_chain_sums and k_chain_left at most
 constexpr int kBatch = 8;                    // logits a thread has under way
 constexpr int kPickThreads = 512;
 constexpr double kChainSlack = 1.0 / 16384;  // 2^-14: four times two sums' bound
@@ -187,7 +187,7 @@ struct Weigh {                               // exp((l - max) / T) of a row's lo
 
 // ---- the draw ----------------------------------------------------------------------------------
 enum ChainMode : int { CM_DONE = 0, CM_P = 1, CM_P_LESS = 2, CM_BOTH = 3, CM_SLOW = 4 };
-struct ChainPlan {                           // of a request, by k_chain_decide
+struct ChainPlan {                           // of a request, by chain_decide
     int mode;                                // weights: none (the token is written), p, p without the refused token,
                                              // max(p - q, 0); or the slow walk
     int acc;                                 // accepted drafts: the row that is drawn from
@@ -197,8 +197,13 @@ struct ChainScratch {
     ChainStat *st;                           // [B][rows][chunks]
     ChainPlan *plan;                         // [B]
     double *sp, *sq, *left;                  // [B][pieces]
+    int piece, pieces;                       // logits of a piece, pieces of a row
 };
-__host__ __device__ inline int chain_pieces(int V) { return (V + kPiece - 1) / kPiece; }
+// Pieces of 4,096 logits, or of half while they leave SMs idle: for one request's four drafts 18 against 21 us
+// (a quarter: 20), for 32 requests 88 against 81.
+inline int chain_piece(int B, int V) {
+    return (long long)B * ((V + kPieceMost - 1) / kPieceMost) < 2 * 148 ? kPieceMost / 2 : kPieceMost;
+}
 
 SP_DEVINL Weigh chain_weigh(const ChainArgs &a, int b, double *tab) {
     if (threadIdx.x < 64) tab[threadIdx.x] = c_exp_tab[threadIdx.x];
@@ -224,18 +229,20 @@ SP_DEVINL void cta_sums(double &x, double &y, double (*s_sum)[THREADS / 32]) {
     }
 }
 
-constexpr int kDecideThreads = 256;
+struct DecideShared {
+    ChainStat row[2 * kChainMaxDrafts + 1];
+    int dec[kChainMaxDrafts];
+};
+// The walk along request b's chain, by a whole CTA; `write`: the plan and every token but the drawn one as well.
 template <typename T>
-__global__ void __launch_bounds__(kDecideThreads) k_chain_decide(ChainArgs a, ChainScratch sc) {
-    __shared__ ChainStat s_row[2 * kChainMaxDrafts + 1];
-    __shared__ double s_tab[64];
-    __shared__ int s_dec[kChainMaxDrafts];
-    griddep_launch_dependents();
-    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+SP_DEVINL ChainPlan chain_decide(const ChainArgs &a, const ChainScratch &sc, int b, const Weigh &weigh, DecideShared &sh,
+                                 bool write) {
+    ChainStat *s_row = sh.row;
+    int *s_dec = sh.dec;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rows = chain_rows(a), chunks = chain_chunks(a.V), cnt = chain_count(a, b);
     const double inv_t = chain_inv_t(a, b);
     const float k2 = chain_k2(a, b);
-    const Weigh weigh = chain_weigh(a, b, s_tab);
     const int *tokens = a.tokens + (size_t)b * a.n;
     // thread i decides draft i: its token, and the token's logits, do not wait for the statistics
     int x = -1;
@@ -251,7 +258,7 @@ __global__ void __launch_bounds__(kDecideThreads) k_chain_decide(ChainArgs a, Ch
     }
     griddep_wait();
     // the rows' statistics: a warp per row, lanes over the chunks
-    for (int r = warp; r < rows; r += kDecideThreads / 32) {
+    for (int r = warp; r < rows; r += kPieceThreads / 32) {
         ChainStat s{0.f, -INFINITY, INT_MAX, 0};
         if (r <= a.n ? r <= cnt : r - a.n - 1 < cnt) {
             const ChainStat *c = sc.st + ((size_t)b * rows + r) * chunks;
@@ -295,14 +302,15 @@ __global__ void __launch_bounds__(kDecideThreads) k_chain_decide(ChainArgs a, Ch
     else if (inv_t == 0.0) pick = s_row[acc].first;
     else if (!refused || (a.draft && plan.mq == -INFINITY)) plan.mode = CM_P;    // a drafter's empty row takes nothing away
     else plan.mode = a.draft ? CM_BOTH : CM_P_LESS;
-    if (tid == 0) sc.plan[b] = plan;
-    if (plan.mode != CM_SLOW) {
+    if (write && tid == 0) sc.plan[b] = plan;
+    if (write && plan.mode != CM_SLOW) {
         int *out = a.out_tokens + (size_t)b * (a.n + 1);
-        for (int i = tid; i <= a.n; i += kDecideThreads)
+        for (int i = tid; i <= a.n; i += kPieceThreads)
             if (i != acc) out[i] = i < acc ? tokens[i] : -1;
             else if (plan.mode == CM_DONE) out[i] = pick;
         if (tid == 0) a.accepted[b] = acc;
     }
+    return plan;
 }
 
 // f(index, logits) of a piece [lo, hi) of row pr and, if given, qr
@@ -328,14 +336,14 @@ SP_DEVINL double left_of(double ep, double ip, double eq, double iq) {
 template <typename T>
 __global__ void __launch_bounds__(kPieceThreads) k_chain_sums(ChainArgs a, ChainScratch sc) {
     __shared__ double s_tab[64], s_sum[2][kPieceThreads / 32];
+    __shared__ DecideShared s_decide;
     griddep_launch_dependents();
-    const int pieces = chain_pieces(a.V), b = blockIdx.x / pieces, k = blockIdx.x - b * pieces;
+    const int pieces = sc.pieces, b = blockIdx.x / pieces, k = blockIdx.x - b * pieces;
     const Weigh weigh = chain_weigh(a, b, s_tab);
     __syncthreads();
-    griddep_wait();
-    const ChainPlan plan = sc.plan[b];
+    const ChainPlan plan = chain_decide<T>(a, sc, b, weigh, s_decide, k == 0);
     if (plan.mode == CM_DONE || plan.mode == CM_SLOW) return;
-    const int lo = k * kPiece, hi = min(a.V, lo + kPiece);
+    const int lo = k * sc.piece, hi = min(a.V, lo + sc.piece);
     const T *pr = chain_row<T>(a, b, plan.acc);
     double sp = 0.0, sq = 0.0;
     if (plan.mode == CM_BOTH) {
@@ -373,7 +381,7 @@ template <typename T>
 __global__ void __launch_bounds__(kPieceThreads) k_chain_left(ChainArgs a, ChainScratch sc) {
     __shared__ double s_tab[64], s_sum[2][kPieceThreads / 32];
     griddep_launch_dependents();
-    const int pieces = chain_pieces(a.V), b = blockIdx.x / pieces, k = blockIdx.x - b * pieces;
+    const int pieces = sc.pieces, b = blockIdx.x / pieces, k = blockIdx.x - b * pieces;
     const Weigh weigh = chain_weigh(a, b, s_tab);
     __syncthreads();
     griddep_wait();
@@ -382,7 +390,7 @@ __global__ void __launch_bounds__(kPieceThreads) k_chain_left(ChainArgs a, Chain
     double sp, sq;
     piece_totals(sc.sp + (size_t)b * pieces, sc.sq + (size_t)b * pieces, pieces, sp, sq);
     const double ip = 1.0 / sp, iq = 1.0 / sq;
-    const int lo = k * kPiece, hi = min(a.V, lo + kPiece);
+    const int lo = k * sc.piece, hi = min(a.V, lo + sc.piece);
     double sum = 0.0, none = 0.0;
     walk_piece<T, kPieceThreads>(chain_row<T>(a, b, plan.acc), chain_row<T>(a, b, a.n + 1 + plan.acc), lo, hi,
                                  [&](int, float x, float y) { sum += left_of(weigh(x, plan.mp), ip, weigh(y, plan.mq), iq); });
@@ -395,7 +403,7 @@ __global__ void __launch_bounds__(kPickThreads) k_chain_pick(ChainArgs a, ChainS
     __shared__ double s_tab[64], s_sum[2][kPickThreads / 32];
     __shared__ int s_pick, s_last;
     const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int pieces = chain_pieces(a.V);
+    const int pieces = sc.pieces;
     const Weigh weigh = chain_weigh(a, b, s_tab);
     const double *u = a.u + (size_t)b * (a.n + 1);
     const int *tokens = a.tokens + (size_t)b * a.n;
@@ -424,7 +432,7 @@ __global__ void __launch_bounds__(kPickThreads) k_chain_pick(ChainArgs a, ChainS
         tx = ty = 0.0;
         for (int k = 0; k < pieces; ++k) {
             double x = 0.0, y = 0.0;
-            walk_piece<T, kPickThreads>(pr, qr, k * kPiece, min(a.V, (k + 1) * kPiece), [&](int, float lp, float lq) {
+            walk_piece<T, kPickThreads>(pr, qr, k * sc.piece, min(a.V, (k + 1) * sc.piece), [&](int, float lp, float lq) {
                 const double ep = weigh(lp, plan.mp), eq = weigh(lq, plan.mq);
                 if (residual) {
                     x += left_of(ep, ip, eq, iq);
@@ -470,8 +478,8 @@ __global__ void __launch_bounds__(kPickThreads) k_chain_pick(ChainArgs a, ChainS
                 plan.mode = CM_P_LESS;
                 if (in && tid == 0) {                        // the refused token out of its piece
                     double y = 0.0;
-                    const int k = x / kPiece;
-                    for (int j = k * kPiece; j < min(a.V, (k + 1) * kPiece); ++j)
+                    const int k = x / sc.piece;
+                    for (int j = k * sc.piece; j < min(a.V, (k + 1) * sc.piece); ++j)
                         if (j != x) y += weigh(to_float(pr[j]), plan.mp);
                     sp[k] = y;
                 }
@@ -528,14 +536,14 @@ __global__ void __launch_bounds__(kPickThreads) k_chain_pick(ChainArgs a, ChainS
         }
         run += __shfl_sync(0xffffffffu, incl, 31);
     }
-    const int lo = own * kPiece, hi = min(a.V, lo + kPiece);
-    constexpr int PER = kPiece / kPickThreads;               // consecutive indices of a thread
+    const int lo = own * sc.piece, hi = min(a.V, lo + sc.piece), per = sc.piece / kPickThreads;
+    constexpr int PER = kPieceMost / kPickThreads;           // consecutive indices of a thread, `per` of them in use
     double w[PER], mine = 0.0;
     int last = -1;
     float lp[PER], lq[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const int j = lo + tid * PER + i;
+        const int j = i < per ? lo + tid * per + i : hi;
         lp[i] = j < hi && j != without ? to_float(pr[j]) : -INFINITY;
         lq[i] = qr && j < hi ? to_float(qr[j]) : -INFINITY;
     }
@@ -544,7 +552,7 @@ __global__ void __launch_bounds__(kPickThreads) k_chain_pick(ChainArgs a, ChainS
         const double ep = weigh(lp[i], plan.mp);
         w[i] = qr ? left_of(ep, ip, weigh(lq[i], plan.mq), iq) : ep;
         mine += w[i];
-        if (w[i] > 0.0) last = lo + tid * PER + i;
+        if (w[i] > 0.0) last = lo + tid * per + i;
     }
     double incl = mine;
     for (int o = 1; o < 32; o <<= 1) {
@@ -562,7 +570,7 @@ __global__ void __launch_bounds__(kPickThreads) k_chain_pick(ChainArgs a, ChainS
         run += w[i];
         if (!found && w[i] > 0.0 && run > want) {
             found = true;
-            atomicMin(&s_pick, lo + tid * PER + i);
+            atomicMin(&s_pick, lo + tid * per + i);
         }
     }
     if (last >= 0) atomicMax(&s_last, last);
@@ -574,8 +582,10 @@ size_t up16(size_t v) { return (v + 15) / 16 * 16; }
 ChainScratch chain_scratch(const ChainArgs &a, void *base) {
     uint8_t *p = static_cast<uint8_t *>(base);
     const auto take = [&](size_t bytes) { uint8_t *q = p; p += up16(bytes); return q; };
-    const size_t pieces = (size_t)a.B * chain_pieces(a.V) * sizeof(double);
     ChainScratch sc{};
+    sc.piece = chain_piece(a.B, a.V);
+    sc.pieces = (a.V + sc.piece - 1) / sc.piece;
+    const size_t pieces = (size_t)a.B * sc.pieces * sizeof(double);
     sc.st = reinterpret_cast<ChainStat *>(take((size_t)a.B * (2 * a.n + 1) * chain_chunks(a.V) * sizeof(ChainStat)));
     sc.plan = reinterpret_cast<ChainPlan *>(take((size_t)a.B * sizeof(ChainPlan)));
     sc.sp = reinterpret_cast<double *>(take(pieces));
@@ -589,8 +599,7 @@ cudaError_t chains_typed(const ChainArgs &a, cudaStream_t s) {
     const ChainScratch sc = chain_scratch(a, a.ws);
     k_chain_stats<T><<<(unsigned)(a.B * chain_rows(a) * chain_chunks(a.V)), kStatThreads, 0, s>>>(a, sc.st);
     cudaError_t e = cudaGetLastError();
-    const dim3 pieces((unsigned)(a.B * chain_pieces(a.V)));
-    if (e == cudaSuccess) e = launch_dependent(k_chain_decide<T>, dim3(a.B), kDecideThreads, 0, s, a, sc);
+    const dim3 pieces((unsigned)(a.B * sc.pieces));
     if (e == cudaSuccess) e = launch_dependent(k_chain_sums<T>, pieces, kPieceThreads, 0, s, a, sc);
     if (e == cudaSuccess && a.draft) e = launch_dependent(k_chain_left<T>, pieces, kPieceThreads, 0, s, a, sc);
     if (e == cudaSuccess) e = launch_dependent(k_chain_pick<T>, dim3(a.B), kPickThreads, 0, s, a, sc);
@@ -605,7 +614,7 @@ size_t chains_workspace(int B, int n, int V) {
     a.n = n;
     a.V = V;
     const ChainScratch sc = chain_scratch(a, nullptr);
-    return reinterpret_cast<size_t>(sc.left) + up16((size_t)B * chain_pieces(V) * sizeof(double));
+    return reinterpret_cast<size_t>(sc.left) + up16((size_t)B * sc.pieces * sizeof(double));
 }
 
 cudaError_t launch_accept_chains(const ChainArgs &a, cudaStream_t s) {

@@ -297,24 +297,20 @@ __global__ void __launch_bounds__(32 * kRowsWarps) k_pages_rows(PagesAttention p
     // the item: its rows, its key range and its pages
     const int n_prefix = pl.prefix_tc ? 0 : pl.prefix_tiles * pl.prefix_splits;
     const int total = total_rows(ba);
-    int item = blockIdx.x, row0, nrows, q0 = 0, own0 = 0, slot, k_lo, k_hi, k_max;
-    const int *table;
-    bool own;
+    int item = blockIdx.x, row0, nrows, q0 = 0, own0 = INT_MAX / 2, slot, k_lo, k_hi, k_own = 0;
+    const int *table, *table_own = nullptr;                  // keys [k_lo, k_hi) of table, then [0, k_own) of table_own
     if (item < n_prefix) {
-        own = false;
         slot = item / pl.prefix_tiles;
         row0 = (item - slot * pl.prefix_tiles) * RT;
         nrows = min(RT, total * G - row0);
-        k_max = ba.prefix_len;
         k_lo = slot * pl.prefix_chunk;
-        k_hi = min(k_max, k_lo + pl.prefix_chunk);
+        k_hi = min(ba.prefix_len, k_lo + pl.prefix_chunk);
         table = ba.prefix;
         if (nrows <= 0) return;
     } else {
-        own = true;
         item -= n_prefix;
-        const int b = item / (pl.own_tiles * pl.own_splits);
-        item -= b * pl.own_tiles * pl.own_splits;
+        const int per = pl.own_tiles * (pl.whole ? 1 : pl.own_splits), b = item / per;
+        item -= b * per;
         const int z = item / pl.own_tiles;
         slot = pl.prefix_slots + z;
         q0 = request_start(ba, b);
@@ -323,8 +319,8 @@ __global__ void __launch_bounds__(32 * kRowsWarps) k_pages_rows(PagesAttention p
         nrows = min(RT, qn * G - row0);
         own0 = len - qn;                                     // token 0's own key
         if (qn > ba.max_q && threadIdx.x == 0) set_status(p.pg.status);
-        int chunk, n;
-        own_chunks(len, pl.own_splits, chunk, n);
+        int chunk = 0, n = 1;
+        if (!pl.whole) own_chunks(len, pl.own_splits, chunk, n);
         if (nrows <= 0) return;
         if (z >= n) {                                        // no such range: nothing to join
             if (threadIdx.x < nrows) {
@@ -334,26 +330,36 @@ __global__ void __launch_bounds__(32 * kRowsWarps) k_pages_rows(PagesAttention p
             }
             return;
         }
-        k_max = len;
-        k_lo = z * chunk;
-        k_hi = min(min(len, k_lo + chunk), own0 + (row0 + nrows - 1) / G + 1);
-        table = ba.tables + (long long)b * ba.table_stride;
+        const int last = min(len, own0 + (row0 + nrows - 1) / G + 1);
+        table_own = ba.tables + (long long)b * ba.table_stride;
+        if (pl.whole) {
+            table = ba.prefix;
+            k_lo = 0;
+            k_hi = ba.prefix_len;
+            k_own = max(0, last);
+        } else {
+            table = table_own;
+            k_lo = z * chunk;
+            k_hi = min(k_lo + chunk, last);
+        }
     }
-    const int ntiles = k_hi > k_lo ? (k_hi - k_lo + KT - 1) / KT : 0;
+    const int ntiles0 = k_hi > k_lo ? (k_hi - k_lo + KT - 1) / KT : 0, ntiles = ntiles0 + (k_own + KT - 1) / KT;
+    const bool own = table == table_own;                     // the first keys are the request's own
     const TC *kb = reinterpret_cast<const TC *>(p.pg.k) + g * p.pg.head_stride;
-    const TC *vb = reinterpret_cast<const TC *>(p.pg.v) + g * p.pg.head_stride;
+    const TC *vbase = reinterpret_cast<const TC *>(p.pg.v) + g * p.pg.head_stride;
     const uint32_t ring = smem_u32(smem) + warp * (kRowsStages * 2 * kRowsTileBytes);
     // The page numbers of 32 pages of the walk, a lane each, so that no tile waits for its own. Pages of whole
     // tiles (the usual case): a tile's rows are slot_stride apart; else every row looks its page up.
     const int ps = p.pg.page_size;
     const bool whole_tiles = ps % KT == 0;
-    int win_first = k_lo / ps, win = 0;
-    const auto fill_window = [&](int first) {
+    int win_first = 0, win_end = 0, win = 0;                 // pages [win_first, win_first + 32) of the keys below win_end
+    const auto fill_window = [&](const int *tab, int first, int hi) {
         win_first = first;
+        win_end = hi;
         const long long key0 = (long long)(first + lane) * ps;
-        win = key0 < k_hi ? __ldg(table + first + lane) : 0;
+        win = key0 < hi ? __ldg(tab + first + lane) : 0;
     };
-    if (ntiles > 0) fill_window(win_first);
+    bool win_own = false;
     // a key's row in its page, -1 on a bad page number (uniform arguments: the window may move)
     const auto row_at = [&](int key, int page) -> long long {
         if ((unsigned)page >= (unsigned)p.pg.n_pages) {
@@ -366,33 +372,41 @@ __global__ void __launch_bounds__(32 * kRowsWarps) k_pages_rows(PagesAttention p
     const auto stage = [&](int tile) {
         const uint32_t ks = ring + (uint32_t)((tile / kRowsWarps) % kRowsStages) * 2 * kRowsTileBytes;
         const uint32_t vs = ks + kRowsTileBytes;
-        const int key0 = k_lo + tile * KT;
+        const bool second = tile >= ntiles0;
+        const int key0 = second ? (tile - ntiles0) * KT : k_lo + tile * KT, hi = second ? k_own : k_hi;
+        const int *tab = second ? table_own : table;
         if (tile < ntiles && whole_tiles) {
             const int pi = key0 / ps;
-            if (pi > win_first + 31) fill_window(pi);
+            if (second != win_own || win_end == 0 || pi > win_first + 31) {
+                win_own = second;
+                fill_window(tab, pi, hi);
+            }
             const long long row = row_at(key0, __shfl_sync(0xffffffffu, win, pi - win_first));
-            const TC *kp = kb + (row < 0 ? 0 : row + lane_off), *vp = vb + (row < 0 ? 0 : row + lane_off);
+            const TC *kp = kb + (row < 0 ? 0 : row + lane_off), *vp = vbase + (row < 0 ? 0 : row + lane_off);
             const long long step = row < 0 ? 0 : 32 / CH * p.pg.slot_stride;
-            const int left = row < 0 ? 0 : k_hi - key0 - lane / CH;    // of the lane's rows, every 32 / CH-th
+            const int left = row < 0 ? 0 : hi - key0 - lane / CH;    // of the lane's rows, every 32 / CH-th
 #pragma unroll
             for (int i = 0; i < KT * CH / 32; ++i) {
                 const uint32_t at = rows_off<HD>(i * (32 / CH) + lane / CH, lane % CH);
                 const bool on = i * (32 / CH) < left;
                 cp16_zfill(ks + at, on ? kp + i * step : kb, on);
-                cp16_zfill(vs + at, on ? vp + i * step : vb, on);
+                cp16_zfill(vs + at, on ? vp + i * step : vbase, on);
             }
         } else if (tile < ntiles) {
-            const int key = min(key0 + min(lane, KT - 1), k_hi - 1), pi = key / ps, last = min(key0 + KT, k_hi) - 1;
-            if (last / ps > win_first + 31) fill_window(key0 / ps);
+            const int key = min(key0 + min(lane, KT - 1), hi - 1), pi = key / ps, last = min(key0 + KT, hi) - 1;
+            if (second != win_own || win_end == 0 || last / ps > win_first + 31) {
+                win_own = second;
+                fill_window(tab, key0 / ps, hi);
+            }
             const long long row = row_at(key, __shfl_sync(0xffffffffu, win, pi - win_first));
 #pragma unroll
             for (int i = 0; i < KT * CH / 32; ++i) {
                 const int r = i * (32 / CH) + lane / CH;
                 const long long o = __shfl_sync(0xffffffffu, row, r);
                 const uint32_t at = rows_off<HD>(r, lane % CH);
-                const bool on = o >= 0 && key0 + r < k_hi;
+                const bool on = o >= 0 && key0 + r < hi;
                 cp16_zfill(ks + at, on ? kb + o + lane % CH * 8 : kb, on);
-                cp16_zfill(vs + at, on ? vb + o + lane % CH * 8 : vb, on);
+                cp16_zfill(vs + at, on ? vbase + o + lane % CH * 8 : vbase, on);
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -424,8 +438,8 @@ __global__ void __launch_bounds__(32 * kRowsWarps) k_pages_rows(PagesAttention p
             }
         }
     }
-    // keys each row sees: below this
-    const int va = own ? min(k_hi, own0 + ra / G + 1) : k_hi, vb_ = own ? min(k_hi, own0 + rb / G + 1) : k_hi;
+    // own keys each row sees: below this
+    const int sa = own0 + ra / G + 1, sb = own0 + rb / G + 1;
     const float sc = p.scale * 1.4426950408889634f;
     float o[NT][4];
 #pragma unroll
@@ -437,7 +451,10 @@ __global__ void __launch_bounds__(32 * kRowsWarps) k_pages_rows(PagesAttention p
         __syncwarp();
         const uint32_t ks = ring + (uint32_t)((tile / kRowsWarps) % kRowsStages) * 2 * kRowsTileBytes;
         const uint32_t vs = ks + kRowsTileBytes;
-        const int j0 = k_lo + tile * KT;
+        // the tile's keys that each row sees: below va, vb
+        const bool second = tile >= ntiles0;
+        const int j0 = second ? (tile - ntiles0) * KT : k_lo + tile * KT, hi = second ? k_own : k_hi;
+        const int va = own || second ? min(hi, sa) : hi, vb = own || second ? min(hi, sb) : hi;
         float s[ST][4];
 #pragma unroll
         for (int nt = 0; nt < ST; ++nt) {
@@ -461,7 +478,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps) k_pages_rows(PagesAttention p
                 s[nt][e] = key < va ? s[nt][e] : -INFINITY;
                 mt[0] = fmaxf(mt[0], s[nt][e]);
                 if constexpr (!kSplit) {
-                    s[nt][2 + e] = key < vb_ ? s[nt][2 + e] : -INFINITY;
+                    s[nt][2 + e] = key < vb ? s[nt][2 + e] : -INFINITY;
                     mt[1] = fmaxf(mt[1], s[nt][2 + e]);
                 }
             }
@@ -665,6 +682,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) k_pages_merge(PagesAttention
 constexpr int kSms = 148;
 constexpr int kTcMinRows = 32;
 constexpr int kTcMinOwnRows = 64;
+constexpr int kWholeValues = 40960, kWholeCtas = 2 * kSms;
 // measured on k_pages_tc: a CTA's start and end, a key tile of two row tiles, of one (the alternate walk), and
 // k_pages_rows' rate over own keys
 constexpr double kTcFixedUs = 8.0, kTcTileUs = 1.8, kTcAltTileUs = 1.0, kOwnBytesPerUs = 4.5e6;
@@ -681,6 +699,15 @@ PagesPlan plan_attention(const PagesAttention &p) {
     if (fits && bound > 0 && own_rows > 128 && rows * nkv / pair >= 96) {
         pl.whole = pl.own_tc = 1;
         pl.own_tiles = (int)up(own_rows, pair);
+        pl.slots = 1;
+        return pl;
+    }
+    // few requests and a walk of at most 5 tiles a warp: one launch and no join (4 requests, 602 keys of 64
+    // dims: 8.0 us on the GPU against 6.9 in two launches, but 10.2 a call in a loop against 13.0)
+    const long long small_tiles = up(own_rows, rt);
+    if (ba.prefix_len > 0 && (ba.prefix_len + bound) * p.pg.hd <= kWholeValues && ba.B * small_tiles * nkv <= kWholeCtas) {
+        pl.whole = 1;
+        pl.own_tiles = (int)small_tiles;
         pl.slots = 1;
         return pl;
     }
@@ -735,7 +762,7 @@ cudaError_t attention_typed(const PagesAttention &p, PagesPlan pl, cudaStream_t 
         if (e != cudaSuccess || pl.whole) return e;
     }
     const int items = (pl.prefix_tc ? 0 : pl.prefix_tiles * pl.prefix_splits) +
-                      (pl.own_tc ? 0 : p.ba.B * pl.own_tiles * pl.own_splits);
+                      (pl.own_tc ? 0 : p.ba.B * pl.own_tiles * (pl.whole ? 1 : pl.own_splits));
     cudaError_t e = raise_smem(k_pages_rows<HD, TQ, TC>, kRowsSmem);
     if (e != cudaSuccess) return e;
     // k_pages_rows does not read what k_pages_tc writes: it starts beside it (and ends after it, which is what

@@ -99,6 +99,7 @@ struct PagesPlan {
     int prefix_tiles, prefix_splits, prefix_chunk, prefix_slots, prefix_tc, prefix_alt;
     int own_tiles, own_splits, own_tc, own_alt;
     int whole;                                               // own_tiles over the prefix and the own keys, no partials
+                                                             // (own_tc: by k_pages_tc, else by k_pages_rows)
     int slots;                                               // partials per (token, head); 1: no merge
     float *acc, *ml;                                         // [slots][T][heads][hd], [slots][T][heads][m, l]
 };

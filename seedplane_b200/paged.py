@@ -24,8 +24,10 @@ from typing import Optional
 import torch
 
 from . import _native as N
-from .engine import _stream
 
+# the current stream's handle by device index, without a Stream object around it
+_raw_stream = torch._C._cuda_getCurrentRawStream
+# The checks below cost as much as a small call's kernels: the common case of each is tested first, in few steps.
 _TYPES = {torch.float32: N.SP_F32, torch.float16: N.SP_F16, torch.bfloat16: N.SP_BF16}
 
 
@@ -71,6 +73,9 @@ class PagedKV:
                 slot_stride=k.stride(3), n_pages=self.n_pages, page_size=self.page_size, kv_heads=self.kv_heads,
                 head_dim=self.head_dim, dtype=_TYPES[k.dtype], status_dev=self._word.data_ptr()))
         self.layer_array = (N.SpPages * self.layers)(*self._layer)
+        self._ref = [C.byref(c) for c in self._layer]
+        # what a workspace's size depends on
+        self._key = (self.n_pages, self.page_size, self.kv_heads, k.dtype, k.stride()[1:])
 
     def status(self):
         """Raise if a kernel met a bad page number, length or position since the last check (waits
@@ -113,7 +118,8 @@ class PageBatch:
             lens_dev=lens.data_ptr(), tables_dev=tables.data_ptr(), table_stride=tables.stride(0) if b > 1 else tables.shape[1],
             table_width=tables.shape[1], prefix_dev=None if prefix_table is None else prefix_table.data_ptr(),
             prefix_len=self.prefix_len)
-        self._ws = {}                          # workspace bytes by (pages, heads, type): sizes only
+        self._ref = C.byref(self._c)
+        self._ws = {}                          # workspace bytes by (pages' sizes, heads, type)
 
     def _check(self, pages: PagedKV, layer: int):
         if not 0 <= layer < pages.layers:
@@ -128,11 +134,13 @@ def _rows(t: torch.Tensor, name: str, batch: PageBatch, cols: int) -> int:
     """The row stride of a [rows, ...] matrix of `cols` values a row (heads and dims contiguous)."""
     if t.device != batch.device or t.dtype not in _TYPES:
         raise ValueError(f"{name}: fp32, fp16 or bf16 on {batch.device} expected")
-    if t.dim() < 2 or t.shape[0] < batch.tokens or math.prod(t.shape[1:]) != cols:
+    if t.dim() < 2 or t.size(0) < batch.tokens or t.numel() != t.size(0) * cols:
         raise ValueError(f"{name}: [{batch.tokens}, {cols}] expected, not {tuple(t.shape)}")
-    if t.numel() > 0 and (t.stride(-1) != 1 or (t.dim() == 3 and t.shape[1] > 1 and t.stride(1) != t.shape[2]) or t.dim() > 3):
+    if t.is_contiguous():
+        return cols
+    if t.numel() > 0 and (t.stride(-1) != 1 or (t.dim() == 3 and t.size(1) > 1 and t.stride(1) != t.size(2)) or t.dim() > 3):
         raise ValueError(f"{name}: the values of a row must be contiguous")
-    return t.stride(0) if t.shape[0] > 1 else cols
+    return t.stride(0) if t.size(0) > 1 else cols
 
 
 def append(pages: PagedKV, layer: int, batch: PageBatch, qkv: torch.Tensor, heads: int, rope: torch.Tensor, *,
@@ -161,9 +169,9 @@ def append(pages: PagedKV, layer: int, batch: PageBatch, qkv: torch.Tensor, head
     if positions is not None and _int32(positions, "positions", batch.device, 1).numel() < batch.tokens:
         raise ValueError(f"positions: {batch.tokens} entries expected")
     N.check(N.load().sp_pages_append(
-        batch.device.index, pages._layer[layer], batch._c, heads, qkv.data_ptr(), _TYPES[qkv.dtype], xs,
+        batch.device.index, pages._ref[layer], batch._ref, heads, qkv.data_ptr(), _TYPES[qkv.dtype], xs,
         None if bias is None else bias.data_ptr(), rope.data_ptr(), rope.shape[0], 2 * rope.shape[1], int(interleaved),
-        None if positions is None else positions.data_ptr(), q_out.data_ptr(), qs, _stream(batch.device)))
+        None if positions is None else positions.data_ptr(), q_out.data_ptr(), qs, _raw_stream(batch.device.index)))
     return q_out
 
 
@@ -174,29 +182,29 @@ def attention(pages: PagedKV, layer: int, batch: PageBatch, q: torch.Tensor, *, 
     scale: default 1 / sqrt(head_dim); lse: fp32 [tokens, heads] that receives the log-sum-exps. Returns
     out, in q's shape and type. The workspace is allocated here, on the current stream."""
     batch._check(pages, layer)
-    if q.dim() != 3 or q.shape[2] != pages.head_dim:
+    if q.dim() != 3 or q.size(2) != pages.head_dim:
         raise ValueError(f"q: [{batch.tokens}, heads, {pages.head_dim}] expected, not {tuple(q.shape)}")
-    heads = q.shape[1]
+    heads = q.size(1)
     qs = _rows(q, "q", batch, heads * pages.head_dim)
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     os_ = _rows(out, "out", batch, heads * pages.head_dim)
     if out.dtype != q.dtype:
         raise ValueError("out must have q's type")
-    if lse is not None and (lse.dtype != torch.float32 or lse.device != batch.device or lse.shape != (q.shape[0], heads) or
+    if lse is not None and (lse.dtype != torch.float32 or lse.device != batch.device or lse.shape != (q.size(0), heads) or
                             not lse.is_contiguous()):
         raise ValueError(f"lse: contiguous fp32 [{q.shape[0]}, {heads}] expected")
-    lib, c, dt = N.load(), pages._layer[layer], _TYPES[q.dtype]
-    key = (pages.n_pages, pages.page_size, pages.kv_heads, pages.k.dtype, pages.k.stride(), heads, dt)
+    lib, c, dt = N.load(), pages._ref[layer], _TYPES[q.dtype]
+    key = (pages._key, heads, dt)
     need = batch._ws.get(key)
     if need is None:
-        need = lib.sp_pages_attention_workspace(c, batch._c, heads, dt)
+        need = lib.sp_pages_attention_workspace(c, batch._ref, heads, dt)
         if need < 0:
             N.check(need)
         batch._ws[key] = need
     ws = torch.empty(need, dtype=torch.uint8, device=batch.device) if need else None
     N.check(lib.sp_pages_attention(
-        batch.device.index, c, batch._c, heads, q.data_ptr(), dt, qs, scale if scale is not None else pages.head_dim ** -0.5,
+        batch.device.index, c, batch._ref, heads, q.data_ptr(), dt, qs, scale if scale is not None else pages.head_dim ** -0.5,
         out.data_ptr(), os_, None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), need,
-        _stream(batch.device)))
+        _raw_stream(batch.device.index)))
     return out

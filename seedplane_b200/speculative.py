@@ -272,42 +272,45 @@ def accept_chains(target_logits, draft_logits, drafts, u, *, counts=None, temper
     the first refused row, or from the last row. Returns (tokens int32 [B, n + 1]: the accepted ones, the
     drawn one, then -1; accepted int32 [B]); `out`: that pair's tensors to write into."""
     import torch
-    from . import _native as N
-    from .engine import _stream
+    from .paged import N, _TYPES, _raw_stream
     dev = target_logits.device
-    types = {torch.float32: N.SP_F32, torch.float16: N.SP_F16, torch.bfloat16: N.SP_BF16}
-    if target_logits.dim() != 3 or not target_logits.is_cuda or target_logits.dtype not in types or \
-            target_logits.stride(2) != 1:
+    dtype = _TYPES.get(target_logits.dtype)
+    if target_logits.dim() != 3 or not target_logits.is_cuda or dtype is None or target_logits.stride(2) != 1:
         raise ValueError("target_logits: fp32, fp16 or bf16 [B, n + 1, V] on a CUDA device, rows contiguous, expected")
     B, n1, V = target_logits.shape
     n = n1 - 1
-    if draft_logits is not None and (draft_logits.shape != (B, n, V) or draft_logits.dtype != target_logits.dtype or
-                                     draft_logits.device != dev or (n > 0 and draft_logits.stride(2) != 1)):
-        raise ValueError(f"draft_logits: [{B}, {n}, {V}] like target_logits expected")
+    draft, dbs, dld = None, 0, 0
+    if draft_logits is not None:
+        if draft_logits.shape != (B, n, V) or draft_logits.dtype != target_logits.dtype or draft_logits.device != dev or \
+                (n > 0 and draft_logits.stride(2) != 1):
+            raise ValueError(f"draft_logits: [{B}, {n}, {V}] like target_logits expected")
+        draft, dbs, dld = draft_logits.data_ptr(), draft_logits.stride(0), draft_logits.stride(1)
 
-    def need(t, name, dtype, shape):
-        if t.dtype != dtype or t.device != dev or t.shape != shape or not t.is_contiguous():
-            raise ValueError(f"{name}: contiguous {dtype} {list(shape)} on {dev} expected")
+    def need(t, name, want, shape):
+        if t.dtype != want or t.device != dev or t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"{name}: contiguous {want} {list(shape)} on {dev} expected")
         return t.data_ptr()
 
+    drafts_at = need(drafts, "drafts", torch.int32, (B, n))
+    u_at = need(u, "u", torch.float64, (B, n1))
+    counts_at = None if counts is None else need(counts, "counts", torch.int32, (B,))
     if temperature is not None and not isinstance(temperature, torch.Tensor):
         temperature = torch.full((B,), float(temperature), dtype=torch.float32, device=dev)
-    if out is None:
-        out = (torch.empty((B, n1), dtype=torch.int32, device=dev), torch.empty(B, dtype=torch.int32, device=dev))
+    temperature_at = None if temperature is None else need(temperature, "temperature", torch.float32, (B,))
     lib = N.load()
     size = lib.sp_accept_chains_workspace(B, n, V)
     if size < 0:
         N.check(size)
-    ws = torch.empty(max(1, size), dtype=torch.uint8, device=dev)
+    ws = u.new_empty(size // 8 + 1)
+    if out is None:
+        out = drafts.new_empty((B, n1)), drafts.new_empty((B,))
+        tokens_at, accepted_at = out[0].data_ptr(), out[1].data_ptr()
+    else:
+        tokens_at = need(out[0], "out tokens", torch.int32, (B, n1))
+        accepted_at = need(out[1], "out accepted", torch.int32, (B,))
     N.check(lib.sp_accept_chains(
-        dev.index, B, n, V, target_logits.data_ptr(), target_logits.stride(0), target_logits.stride(1),
-        None if draft_logits is None else draft_logits.data_ptr(), 0 if draft_logits is None else draft_logits.stride(0),
-        0 if draft_logits is None else draft_logits.stride(1), types[target_logits.dtype],
-        need(drafts, "drafts", torch.int32, (B, n)), None if counts is None else need(counts, "counts", torch.int32, (B,)),
-        need(u, "u", torch.float64, (B, n1)),
-        None if temperature is None else need(temperature, "temperature", torch.float32, (B,)),
-        need(out[0], "out tokens", torch.int32, (B, n1)), need(out[1], "out accepted", torch.int32, (B,)),
-        ws.data_ptr(), ws.numel(), _stream(dev)))
+        dev.index, B, n, V, target_logits.data_ptr(), target_logits.stride(0), target_logits.stride(1), draft, dbs, dld, dtype,
+        drafts_at, counts_at, u_at, temperature_at, tokens_at, accepted_at, ws.data_ptr(), size, _raw_stream(dev.index)))
     return out
 
 
