@@ -31,8 +31,9 @@ namespace {
 
 constexpr int kTcKeys = 128;                 // keys of a tile
 constexpr int kTcRows = 128;                 // rows of a row tile
-constexpr int kTcThreads = 384;              // warps 10, 11 only fill the third warpgroup
-constexpr int kTcProducer = 8, kTcMma = 9;   // warps
+constexpr int kTcSoftmax = 512;              // threads: two row tiles x two halves of the columns x 128 rows
+constexpr int kTcThreads = kTcSoftmax + 64;
+constexpr int kTcProducer = 16, kTcMma = 17; // warps
 constexpr int kTcStages = 4;
 constexpr uint32_t kTcSpin = 1u << 22;
 constexpr float kTcGrow = 8.0f;              // log2 of the growth a running maximum may lag behind
@@ -100,9 +101,6 @@ SP_DEVINL float max3(float a, float b, float c) {             // NaN is passed o
 SP_DEVINL void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-SP_DEVINL void bulk_s2g(void *dst, uint32_t src, uint32_t bytes) {
-    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
-}
 SP_DEVINL bool elect_one() {
     uint32_t p;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
@@ -159,6 +157,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     __shared__ __align__(8) TcBarriers bar;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
+    __shared__ float s_swap[2][2][kTcRows];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const PageBatchView &ba = p.ba;
     const int g = blockIdx.y, G = p.nh / p.pg.nkv;
@@ -237,10 +236,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_init(&bar.full[i], 1);
             mbar_init(&bar.empty[i], 1);
         }
-        mbar_init(&bar.q_full, 256);
+        mbar_init(&bar.q_full, kTcSoftmax);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar.s_full[i], 1);
-            mbar_init(&bar.p_full[i], 128);
+            mbar_init(&bar.p_full[i], kTcSoftmax / 2);
             mbar_init(&bar.o_full[i], 1);
         }
         mbar_init(&bar.tail, 1);
@@ -256,11 +255,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     tc_fence_after();
     const uint32_t tmem = s_tmem;
 
-    // 384 threads of 168 registers at launch: the softmax groups take 216, the third 72 (the sum is the same; with
-    // 56 the MMA warp spilled, 188 -> 212 us)
-    if (warp >= kTcProducer) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (warp == kTcProducer) {
+    if (warp == kTcProducer) {
         // ring order: K of the first `lead` tiles, then V of tile i and K of tile i + lead
         const int lead = alt ? 2 : 1;
         int it = 0, tails = 0;
@@ -323,7 +318,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int j = max(0, it - kTcStages); j < it; ++j)
             for (uint32_t k = 0; k < kTcSpin && !mbar_try_wait(&bar.full[j % kTcStages], (uint32_t)(j / kTcStages) & 1u); ++k) {
             }
-        } else if (warp == kTcMma) {
+    } else if (warp == kTcMma) {
         // the whole warp runs the loop, one elected lane issues: control flow and descriptors stay uniform
         if (n > 0 && w.wait_warp(&bar.q_full, 0)) {
             constexpr uint32_t id_s = tc_idesc<TC>(kTcKeys, false), id_o = tc_idesc<TC>(HD, true);
@@ -367,7 +362,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     for (int part = 0; part < (kSplit ? 2 : 1); ++part)
 #pragma unroll
                         for (int kk = 0; kk < kTcKeys / 16; ++kk)
-                            mma_ts(tmem + 256 + 128 * q, tmem + 128 * q + 64 * part + 8 * kk, vd + ((kk * 2048) >> 4), id_o,
+                            mma_ts(tmem + 256 + 128 * q, tmem + 128 * q + 32 * (kk >> 1) + 8 * (kk & 1) + 16 * part, vd + ((kk * 2048) >> 4), id_o,
                                    !(first && part + kk == 0));
                 }
                 __syncwarp();
@@ -416,19 +411,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
         }
         __syncwarp();
-        }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        const int grp = warp >> 2;
+        const int grp = warp >> 3, half = (warp >> 2) & 1;
         const TQ *qbase = reinterpret_cast<const TQ *>(p.q);
         // Q rows into swizzled tiles (rows behind the last: zero), a batch of loads under way at once
         const int fill = (alt || nq == 1 ? 1 : 2) * kTcRows * CH;
         constexpr int QB = kSplit ? 4 : 8;
-        for (int i0 = tid; i0 < fill; i0 += 256 * QB) {
+        for (int i0 = tid; i0 < fill; i0 += kTcSoftmax * QB) {
             uint4 v[QB], v2[kSplit ? QB : 1];
 #pragma unroll
             for (int j = 0; j < QB; ++j) {
-                const int i = i0 + 256 * j, r = i / CH, c = i - r * CH, row = row0 + r;
+                const int i = i0 + kTcSoftmax * j, r = i / CH, c = i - r * CH, row = row0 + r;
                 v[j] = make_uint4(0u, 0u, 0u, 0u);
                 if constexpr (kSplit) v2[j] = v[j];
                 if (r < nrows) {
@@ -439,7 +432,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
 #pragma unroll
             for (int j = 0; j < QB; ++j) {
-                const int i = i0 + 256 * j, r = i / CH, c = i - r * CH;
+                const int i = i0 + kTcSoftmax * j, r = i / CH, c = i - r * CH;
                 if (i >= fill) break;
                 const uint32_t at = base + (uint32_t)(r >> 7) * L::kTile + (c >> 3) * L::kHalf + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4);
                 if constexpr (kSplit) {
@@ -472,45 +465,55 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             float m = -INFINITY, l = 0.f;
             uint32_t ph = 0u;
             bool ok = true, any = false;
+            // the two halves of a row's columns: their threads exchange a value through shared memory
+            const auto swap = [&](float v) -> float {
+                s_swap[grp][half][r & 127] = v;
+                asm volatile("bar.sync %0, 64;" ::"r"(1 + grp * 4 + (warp & 3)) : "memory");
+                return s_swap[grp][half ^ 1][r & 127];
+            };
             for (int i = alt ? grp : 0; i < n; i += alt ? 2 : 1) {
-                if (!w.wait_warp(&bar.s_full[grp], ph)) { ok = false; break; }
+                // after an expired wait the walk goes on over whatever is there: every thread keeps to its barriers
+                if (ok) ok = w.wait_warp(&bar.s_full[grp], ph);
                 ph ^= 1u;
                 tc_fence_after();
-                uint32_t s[4][32];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) tmem_ld32_nowait(ts + 32 * k, s[k]);
-                tmem_wait_ld();
-                const int lo = ks.lo(i), lim = min(ks.hi(i), i >= own_tile0 ? seen : INT_MAX) - lo;
-                if (__any_sync(0xffffffffu, lim < kTcKeys)) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
+                const int lo = ks.lo(i), lim = min(ks.hi(i), i >= own_tile0 ? seen : INT_MAX) - lo - 64 * half;
+                const bool cut = __any_sync(0xffffffffu, lim < 64);
+                // 32 columns at a time, read again for the exponentials: half the registers, and four warps a
+                // scheduler instead of two
+                const auto scores = [&](int k, uint32_t (&s)[32]) {
+                    tmem_ld32_nowait(ts + 64 * half + 32 * k, s);
+                    tmem_wait_ld();
+                    if (cut) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
-                            if (32 * k + j >= lim) s[k][j] = 0xff800000u;             // -inf
-                }
-                float mx[4];
+                            if (32 * k + j >= lim) s[j] = 0xff800000u;                // -inf
+                    }
+                };
+                float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    mx[k] = fmaxf(__uint_as_float(s[k][0]), __uint_as_float(s[k][1]));
+                for (int k = 0; k < 2; ++k) {
+                    uint32_t s[32];
+                    scores(k, s);
 #pragma unroll
-                    for (int j = 2; j < 32; j += 2) mx[k] = max3(mx[k], __uint_as_float(s[k][j]), __uint_as_float(s[k][j + 1]));
+                    for (int j = 0; j < 32; j += 4) {
+                        mx[0] = max3(mx[0], __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
+                        mx[1] = max3(mx[1], __uint_as_float(s[j + 2]), __uint_as_float(s[j + 3]));
+                    }
                 }
-                const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+                const float mine = fmaxf(mx[0], mx[1]), mt = fmaxf(mine, swap(mine)) * c;
                 const bool grow = mt > m + kTcGrow || (!any && mt > m);
-                if (any) {
-                    // sfull of this tile came after the products of the tile before: O is at rest
-                    if (__any_sync(0xffffffffu, grow)) {
-                        const float f = grow ? exp2_approx(m - mt) : 1.f;
-                        l *= f;
+                if (any && __any_sync(0xffffffffu, grow)) {
+                    // s_full of this tile came after the products of the tile before: O is at rest
+                    const float f = grow ? exp2_approx(m - mt) : 1.f;
+                    l *= f;
 #pragma unroll
-                        for (int k = 0; k < HD / 32; ++k) {
-                            uint32_t o[32];
-                            tmem_ld32_nowait(to + 32 * k, o);
-                            tmem_wait_ld();
+                    for (int k = 0; k < HD / 64; ++k) {
+                        uint32_t o[32];
+                        tmem_ld32_nowait(to + HD / 2 * half + 32 * k, o);
+                        tmem_wait_ld();
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                            tmem_st32(to + 32 * k, o);
-                        }
+                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                        tmem_st32(to + HD / 2 * half + 32 * k, o);
                     }
                 }
                 if (grow) m = mt;
@@ -519,11 +522,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const uint64_t c2 = f2(c, c), m2 = f2(-ms, -ms);
                 uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    uint32_t hi[16], lw[16];
+                for (int k = 0; k < 2; ++k) {
+                    uint32_t s[32], hi[16], lw[16];
+                    scores(k, s);
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
-                        const uint64_t x = fma2((uint64_t)s[k][2 * j] | ((uint64_t)s[k][2 * j + 1] << 32), c2, m2);
+                        const uint64_t x = fma2((uint64_t)s[2 * j] | ((uint64_t)s[2 * j + 1] << 32), c2, m2);
                         const float e0 = exp2_approx(f2_lo(x)), e1 = exp2_approx(f2_hi(x));
                         sum[j & 1] = add2(sum[j & 1], f2(e0, e1));
                         hi[j] = pack2<TC>(e0, e1);
@@ -533,30 +537,35 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             lw[j] = pack2<TC>(e0 - h0, e1 - h1);
                         }
                     }
-                    tmem_st16(ts + 16 * k, hi);
-                    if constexpr (kSplit) tmem_st16(ts + 64 + 16 * k, lw);
+                    // in place of the 32 scores: 16 columns of P, and of its lo half
+                    tmem_st16(ts + 64 * half + 32 * k, hi);
+                    if constexpr (kSplit) tmem_st16(ts + 64 * half + 32 * k + 16, lw);
                 }
                 sum[0] = add2(sum[0], sum[1]);
                 l += f2_lo(sum[0]) + f2_hi(sum[0]);
                 tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive(&bar.p_full[grp]);
+                // the next tile's swap writes what this one read: this tile's MMAs lie between (s_full)
             }
-            // O and the row's statistics. A thread's row goes through shared memory (the tiles are done with once both
-            // groups' products are) and out as one bulk copy: 16-byte stores of 32 rows a warp took 4 us
+            // O and the row's statistics, half of the dims per thread. A warp's 32 half rows go through shared memory
+            // (the tiles are done with once both groups' products are) and out as whole rows: a thread storing its
+            // own row, 16 bytes of 32 rows at a time, took 4 us, a bulk copy per row 2.5
             for (int q = 0; q < nq; ++q)
                 if (ok && (alt ? q < n : n > 0)) ok = w.wait_warp(&bar.o_full[q], 0);
             tc_fence_after();
+            l += swap(l);
             const long long rt = q0 + row / G, hh = g * G + row % G;
             const long long at = ((long long)(slot + (alt ? grp : 0)) * ba.T + rt) * p.nh + hh;
             const bool direct = pl.slots == 1;
             const float inv = l > 0.f ? 1.f / l : 0.f;
-            const uint32_t stage = base + (uint32_t)(grp * kTcRows + (warp & 3) * 32 + lane) * (HD * 4 + 16);
+            constexpr int HALF = HD / 2, STRIDE = HALF * 4 + 16;
+            const uint32_t stage = base + (uint32_t)warp * 32 * STRIDE;
 #pragma unroll
-            for (int k = 0; k < HD / 32; ++k) {
+            for (int k = 0; k < HALF / 32; ++k) {
                 uint32_t o[32];
                 if (any && ok) {
-                    tmem_ld32_nowait(to + 32 * k, o);
+                    tmem_ld32_nowait(to + HALF * half + 32 * k, o);
                     tmem_wait_ld();
                 } else {
 #pragma unroll
@@ -566,30 +575,39 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
                     for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(l == l ? __uint_as_float(o[j]) * inv : l);
                 }
+                const uint32_t mine = stage + lane * STRIDE;
                 if (direct && !kSplit) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         uint32_t v[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) v[i] = pack2<TC>(__uint_as_float(o[8 * j + 2 * i]), __uint_as_float(o[8 * j + 2 * i + 1]));
-                        st_shared16(stage + 64 * k + 16 * j, v[0], v[1], v[2], v[3]);
+                        st_shared16(mine + 64 * k + 16 * j, v[0], v[1], v[2], v[3]);
                     }
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) st_shared16(stage + 128 * k + 16 * j, o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                    for (int j = 0; j < 8; ++j) st_shared16(mine + 128 * k + 16 * j, o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
                 }
             }
-            fence_proxy_async_smem();
-            if (live) {
-                if (direct) {
-                    bulk_s2g(reinterpret_cast<TQ *>(p.out) + rt * p.out_stride + hh * HD, stage, HD * sizeof(TQ));
-                    if (p.lse) p.lse[rt * p.nh + hh] = row_lse(m, l);
-                } else {
-                    bulk_s2g(pl.acc + at * HD, stage, HD * 4);
-                    *reinterpret_cast<float2 *>(pl.ml + at * 2) = make_float2(m, l);
-                }
+            // each lane knows where its own row goes
+            uint8_t *dst = direct ? reinterpret_cast<uint8_t *>(reinterpret_cast<TQ *>(p.out) + rt * p.out_stride + hh * HD + HALF * half)
+                                  : reinterpret_cast<uint8_t *>(pl.acc + at * HD + HALF * half);
+            if (!live) dst = nullptr;
+            __syncwarp();
+            const int per = (direct ? HALF * (int)sizeof(TQ) : HALF * 4) / 16, rows = 32 / per;    // lanes a row, rows at once
+#pragma unroll 4
+            for (int i = 0; i < 32; i += rows) {
+                const int from = i + lane / per, c16 = lane % per * 16;
+                uint8_t *d = reinterpret_cast<uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), from));
+                uint4 v;
+                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(stage + from * STRIDE + c16));
+                if (d) *reinterpret_cast<uint4 *>(d + c16) = v;
             }
-            asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
+            if (live && half == 0) {
+                if (!direct) *reinterpret_cast<float2 *>(pl.ml + at * 2) = make_float2(m, l);
+                else if (p.lse) p.lse[rt * p.nh + hh] = row_lse(m, l);
+            }
             tc_fence_before();
         }
     }
