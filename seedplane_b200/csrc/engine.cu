@@ -1853,7 +1853,8 @@ int check_pages(const sp_pages *pages, const sp_page_batch *batch, int32_t heads
         return fail(SP_ERR_INVALID, "batch: tables into no pages");
     // key numbers, and positions behind the prefix, are 32-bit
     if ((int64_t)batch->prefix_len + (int64_t)batch->table_width * pages->page_size > INT32_MAX - 4096 ||
-        (int64_t)batch->tokens * heads > INT32_MAX / 2)
+        (int64_t)batch->tokens * heads > INT32_MAX / 2 ||
+        (int64_t)batch->batch * (std::min(batch->max_q, batch->tokens) * (int64_t)(heads / pages->kv_heads) / 8 + 1) > INT32_MAX / 64)
         return fail(SP_ERR_CAPACITY, "batch: more keys or rows than 32-bit numbers count");
     pg = PagesView{pages->k_dev, pages->v_dev, pages->page_stride, pages->head_stride, pages->slot_stride,
                    pages->n_pages, pages->page_size, pages->kv_heads, pages->head_dim, pages->status_dev};

@@ -186,6 +186,56 @@ def test_attention_of_larger_batches_strides_and_scales(dt, prefix, batch):
     check_attention(s, q, got, scale=0.21)
 
 
+@pytest.mark.parametrize("dt,cache", [(F16, F16), (BF16, BF16), (F32, F16)])
+@pytest.mark.parametrize("prefix", [1, 15, 16, 17, 127, 128, 129, 257])
+def test_attention_of_short_prefixes_under_many_rows(prefix, dt, cache):
+    for batch, nh, nkv, hd, page in ((40, 14, 2, 64, 16), (9, 12, 2, 128, 32), (23, 28, 4, 128, 8)):
+        s = oracle.make_batch(q=[1] * batch, lens=[1 + (7 * i) % 33 for i in range(batch)], prefix=prefix, page=page, nkv=nkv, hd=hd,
+                              dtype=cache, seed=prefix)
+        x, got = run_attention(s, nh, dt)
+        check_attention(s, x, got)
+
+
+@pytest.mark.parametrize("dt,cache,nh,nkv,hd", [(F16, F16, 28, 4, 128), (BF16, BF16, 14, 2, 64), (F32, F16, 12, 2, 128),
+                                                (F32, F16, 16, 8, 64)])
+@pytest.mark.parametrize("prefix,page", [(130, 64), (0, 16), (31, 128)])
+def test_attention_of_packed_prompts(dt, cache, nh, nkv, hd, prefix, page):
+    """Rows enough for a row tile to walk the prefix and its request's own keys by itself."""
+    q = [300, 1, 250, 0, 420, 129, 512, 40]
+    s = oracle.make_batch(q=q, lens=[n + (17 * i) % 90 for i, n in enumerate(q)], prefix=prefix, page=page, nkv=nkv, hd=hd, dtype=cache,
+                          tail_rows=2)
+    out = torch.full((s["rows"], nh, hd), 7.0, device="cuda", dtype=dt)
+    lse = torch.full((s["rows"], nh), 5.0, device="cuda")
+    x, got = run_attention(s, nh, dt, out=out, lse=lse)
+    check_attention(s, x, got, lse)
+    assert (got[s["start"][-1]:] == 7.0).all()
+
+
+def test_attention_of_values_that_a_wrong_order_would_show():
+    """Keys far apart in size and values that name their key: the row of the largest key comes back exactly."""
+    for prefix, own in ((300, 40), (128, 200), (0, 77)):
+        s = oracle.make_batch(q=[1, 1], lens=[own, own + 3], prefix=prefix, page=16, nkv=1, hd=64, dtype=F16, garbage=0.0)
+        s["k"].zero_()
+        s["v"].zero_()
+        n = prefix + own
+        for b in range(2):
+            for j in range(prefix if b else 0, prefix + s["len"][b]):
+                page = s["prefix_pages"][j // 16] if j < prefix else s["own"][b][(j - prefix) // 16]
+                at = j % 16 if j < prefix else (j - prefix) % 16
+                s["k"][0, page, 0, at, 0] = 100.0 if j == (37 * (b + 1)) % n else 0.0
+                s["v"][0, page, 0, at] = float(j % 251)
+        from seedplane_b200 import paged
+        pages, batch = setup(s)
+        x = torch.zeros(2, 2, 64, device="cuda", dtype=F16)
+        x[:, :, 0] = 50.0
+        got = paged.attention(pages, 0, batch, x)
+        hot = [j for j in (37 % n, 74 % n)]
+        if prefix == 0:
+            assert (got[0] == float(hot[0] % 251)).all() and (got[1] == float(hot[1] % 251)).all()
+        else:                                            # the second request's hot key may lie in the shared prefix
+            check_attention(s, x, got)
+
+
 def test_attention_of_large_scores_and_infinite_keys_out_of_sight():
     """Scores of several hundred (one key wins), and infinities in slots behind a request's last key."""
     s = oracle.make_batch(q=[1, 2, 1], lens=[40, 41, 42], prefix=130, page=16, nkv=2, hd=64, dtype=F16, garbage=float("inf"))

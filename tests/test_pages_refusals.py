@@ -46,7 +46,8 @@ BAD_BATCH = [(dict(batch=0), N.SP_ERR_INVALID), (dict(batch=-1), N.SP_ERR_INVALI
              (dict(tokens=-1), N.SP_ERR_INVALID), (dict(lens_dev=None), N.SP_ERR_INVALID), (dict(tables_dev=None), N.SP_ERR_INVALID),
              (dict(table_stride=3), N.SP_ERR_INVALID), (dict(prefix_dev=None), N.SP_ERR_INVALID),
              (dict(prefix_len=-1), N.SP_ERR_INVALID), (dict(prefix_len=2 ** 31 - 1), N.SP_ERR_CAPACITY),
-             (dict(tokens=2 ** 30), N.SP_ERR_CAPACITY)]
+             (dict(tokens=2 ** 30), N.SP_ERR_CAPACITY), (dict(batch=2 ** 30), N.SP_ERR_CAPACITY),
+             (dict(batch=2 ** 20, tokens=2 ** 20, max_q=2 ** 20), N.SP_ERR_CAPACITY)]
 
 
 @pytest.mark.parametrize("change,code", BAD_PAGES)
@@ -71,8 +72,12 @@ def test_bad_arguments(lib):
         assert append(lib, p, b, **bad) == N.SP_ERR_INVALID, bad
     assert append(lib, p, b, dtype=N.SP_BF16) == N.SP_ERR_UNSUPPORTED
     for bad in (dict(q=None), dict(out=None), dict(qs=100), dict(os_=4 * 64 + 1), dict(q=PTR + 8), dict(scale=0.0),
-                dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(size=8), dict(ws=None), dict(ws=PTR + 4)):
+                dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf"))):
         assert attention(lib, p, b, **bad) == N.SP_ERR_INVALID, bad
+    longer = batch(prefix_len=20000)                     # key ranges whose results are joined need a workspace
+    assert lib.sp_pages_attention_workspace(p, longer, 4, N.SP_F16) > 8
+    for bad in (dict(size=8), dict(ws=None), dict(ws=PTR + 4)):
+        assert attention(lib, p, longer, **bad) == N.SP_ERR_INVALID, bad
     assert attention(lib, p, b, dtype=N.SP_BF16) == N.SP_ERR_UNSUPPORTED
     assert attention(lib, pages(dtype=N.SP_BF16), b, dtype=N.SP_F32) == N.SP_ERR_UNSUPPORTED
     # nothing to do is fine, whatever the pointers
