@@ -18,10 +18,10 @@
 // The pieces spread the requests' fp64 work (four exponentials a token after a refusal, else one) over all SMs; a
 // cluster of 8 CTAs per request for the last four took 43 us for 32 requests and 36 for 48 without a drafter, these
 // 40 and 24.
-// How far k_chain_stats' sum may be off, relatively: z = (l - max) / T in base 2 carries two roundings and 1 / T a
-// third (3 2^-24 |z|, and terms below 2^-60 of the largest weigh nothing: 2^-16.5 at |z| = 60), the
-// exponential 2^-22, the sums over a thread's 32 terms, a warp, a CTA and the chunks at most 60 2^-24: below
-// 2^-16 together; u q / p takes two such sums.
+// How far k_chain_stats' sum may be off, relatively: z = (l - max) / T in base 2 carries four roundings (1 / T has
+// two), so a term is off by 4 2^-24 |z| ln 2, and terms below 2^-60 of the largest weigh nothing: 2^-16.6 at
+// |z| = 60; the exponential 2^-22; the sums over a thread's 64 terms, a warp, a CTA and the chunks at most
+// 92 2^-24: below 2^-15.9 together. u q / p takes two such sums: 2^-14.9.
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -33,14 +33,13 @@ namespace sp {
 
 namespace {
 
-constexpr int kStatThreads = 256;
-constexpr int kStatChunk = 8192;             // logits per CTA of k_chain_stats
-constexpr int kStatPer = kStatChunk / kStatThreads;
+constexpr int kStatThreads = 128;
+constexpr int kStatMost = 64;                // logits per thread of k_chain_stats at most
 constexpr int kPieceThreads = 256;
 constexpr int kPieceMost = 4096;             // logits per CTA of k_chain_sums and k_chain_left at most
 constexpr int kBatch = 8;                    // logits a thread has under way
 constexpr int kPickThreads = 512;
-constexpr double kChainSlack = 1.0 / 16384;  // 2^-14: four times two sums' bound
+constexpr double kChainSlack = 1.0 / 16384;  // 2^-14, above what two sums may be off
 
 struct ChainStat {                           // of a chunk or a row
     float sum;                               // sum of exp((l - max) / T)
@@ -85,13 +84,19 @@ SP_DEVINL const T *chain_row(const ChainArgs &a, int b, int r) {
                     : static_cast<const T *>(a.draft) + b * a.draft_bs + (long long)(r - a.n - 1) * a.draft_ld;
 }
 __host__ __device__ inline int chain_rows(const ChainArgs &a) { return a.draft ? 2 * a.n + 1 : a.n + 1; }
-__host__ __device__ inline int chain_chunks(int V) { return (V + kStatChunk - 1) / kStatChunk; }
+// Logits per CTA of k_chain_stats: 64 a thread, or 32 while that leaves SMs idle (32 requests' five drafts 79 ->
+// 75 us with 64, one request's four 17 -> 19).
+inline int chain_chunk(int rows, int V) {
+    const int most = kStatMost * kStatThreads;
+    return (long long)rows * ((V + most - 1) / most) < 4 * 148 ? most / 2 : most;
+}
 
-template <typename T>
+template <typename T, int PER>
 __global__ void __launch_bounds__(kStatThreads) k_chain_stats(ChainArgs a, ChainStat *st) {
+    constexpr int kStatPer = PER, kStatChunk = PER * kStatThreads;
     __shared__ ChainStat s_st[kStatThreads / 32];
     griddep_launch_dependents();
-    const int chunks = chain_chunks(a.V), rows = chain_rows(a), tid = threadIdx.x;
+    const int chunks = (a.V + kStatChunk - 1) / kStatChunk, rows = chain_rows(a), tid = threadIdx.x;
     const int br = blockIdx.x / chunks, chunk = blockIdx.x - br * chunks, b = br / rows, r = br - b * rows;
     const int cnt = chain_count(a, b);
     if (r <= a.n ? r > cnt : r - a.n - 1 >= cnt) return;     // a row behind the request's drafts
@@ -198,6 +203,7 @@ struct ChainScratch {
     ChainPlan *plan;                         // [B]
     double *sp, *sq, *left;                  // [B][pieces]
     int piece, pieces;                       // logits of a piece, pieces of a row
+    int chunk, chunks;                       // likewise of the statistics
 };
 // Pieces of 4,096 logits, or of half while they leave SMs idle: for one request's four drafts 18 against 21 us
 // (a quarter: 20), for 32 requests 88 against 81.
@@ -240,7 +246,7 @@ SP_DEVINL ChainPlan chain_decide(const ChainArgs &a, const ChainScratch &sc, int
     ChainStat *s_row = sh.row;
     int *s_dec = sh.dec;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int rows = chain_rows(a), chunks = chain_chunks(a.V), cnt = chain_count(a, b);
+    const int rows = chain_rows(a), chunks = sc.chunks, cnt = chain_count(a, b);
     const double inv_t = chain_inv_t(a, b);
     const float k2 = chain_k2(a, b);
     const int *tokens = a.tokens + (size_t)b * a.n;
@@ -583,10 +589,12 @@ ChainScratch chain_scratch(const ChainArgs &a, void *base) {
     uint8_t *p = static_cast<uint8_t *>(base);
     const auto take = [&](size_t bytes) { uint8_t *q = p; p += up16(bytes); return q; };
     ChainScratch sc{};
+    sc.chunk = chain_chunk(a.B * (2 * a.n + 1), a.V);
+    sc.chunks = (a.V + sc.chunk - 1) / sc.chunk;
     sc.piece = chain_piece(a.B, a.V);
     sc.pieces = (a.V + sc.piece - 1) / sc.piece;
     const size_t pieces = (size_t)a.B * sc.pieces * sizeof(double);
-    sc.st = reinterpret_cast<ChainStat *>(take((size_t)a.B * (2 * a.n + 1) * chain_chunks(a.V) * sizeof(ChainStat)));
+    sc.st = reinterpret_cast<ChainStat *>(take((size_t)a.B * (2 * a.n + 1) * sc.chunks * sizeof(ChainStat)));
     sc.plan = reinterpret_cast<ChainPlan *>(take((size_t)a.B * sizeof(ChainPlan)));
     sc.sp = reinterpret_cast<double *>(take(pieces));
     sc.sq = reinterpret_cast<double *>(take(pieces));
@@ -597,7 +605,11 @@ ChainScratch chain_scratch(const ChainArgs &a, void *base) {
 template <typename T>
 cudaError_t chains_typed(const ChainArgs &a, cudaStream_t s) {
     const ChainScratch sc = chain_scratch(a, a.ws);
-    k_chain_stats<T><<<(unsigned)(a.B * chain_rows(a) * chain_chunks(a.V)), kStatThreads, 0, s>>>(a, sc.st);
+    const unsigned stats = (unsigned)(a.B * chain_rows(a) * sc.chunks);
+    if (sc.chunk == kStatMost * kStatThreads)
+        k_chain_stats<T, kStatMost><<<stats, kStatThreads, 0, s>>>(a, sc.st);
+    else
+        k_chain_stats<T, kStatMost / 2><<<stats, kStatThreads, 0, s>>>(a, sc.st);
     cudaError_t e = cudaGetLastError();
     const dim3 pieces((unsigned)(a.B * sc.pieces));
     if (e == cudaSuccess) e = launch_dependent(k_chain_sums<T>, pieces, kPieceThreads, 0, s, a, sc);

@@ -238,10 +238,10 @@ cudaError_t append_typed(const PagesAppend &p, cudaStream_t s) {
 // read once for 16 rows of the batch; of one request's for its own keys. fp32 queries: 8 rows, tile
 // row i = fp16 hi of row i's q, 8 + i its fp16 lo, and the probabilities likewise.
 // Bound by the K / V stream. Each of the 4 warps walks every fourth tile of 2,048 / HD keys through a
-// private ring of shared memory (cp.async, three tiles deep, no block barrier in the loop) and
+// private ring of shared memory (cp.async, two tiles deep: three CTAs a SM; no block barrier in the loop) and
 // keeps its own (m, l, O); the warps' results are joined at the end, the key ranges' by
 // k_pages_merge.
-constexpr int kRowsWarps = 4, kRowsStages = 3;
+constexpr int kRowsWarps = 4, kRowsStages = 2;
 constexpr int kRowsTileBytes = 4096;                         // K (or V) rows of one warp's tile
 constexpr int kRowsSmem = kRowsWarps * kRowsStages * 2 * kRowsTileBytes;
 
