@@ -96,6 +96,26 @@ def test_identical_distributions_accept_everything_and_extreme_numbers():
     assert run(target, draft, drafts, u) == oracle.chains(target, draft, drafts, u, None, None)
 
 
+@pytest.mark.parametrize("drafter", [True, False])
+def test_numbers_next_to_the_border_are_decided_in_64_bits(drafter):
+    """u q(x) a millionth under or over p(x), drafts on both sides of it along one chain, and a draw after each."""
+    B, n, V = 6, 3, 5000
+    target, draft, drafts, u = case(B, n, V, torch.float32, seed=17, spread=1.0, near=0.3)
+    if not drafter:
+        draft = None
+        drafts = target[:, :n].argmax(-1).int()
+    temperature = torch.full((B,), 0.7)
+    for b in range(B):
+        for i in range(n):
+            x = int(drafts[b, i])
+            dist = lambda row: torch.softmax(row.double() / 0.7, 0)  # noqa: E731
+            p, q = float(dist(target[b, i])[x]), float(dist(draft[b, i])[x]) if drafter else 1.0
+            u[b, i] = min(p / q, 0.999999) * (1 + (1e-6 if (b >> i) & 1 else -1e-6))
+    got = run(target, draft, drafts, u, None, temperature)
+    assert got == oracle.chains(target, draft, drafts, u, None, temperature)
+    assert set(got[1]) >= {0, 1, 2} if not drafter else True
+
+
 def test_strided_rows_and_rows_behind_the_counts_are_not_read():
     target, draft, drafts, u = case(3, 3, 999, torch.float32, seed=13)
     counts = torch.tensor([1, 3, 0], dtype=torch.int32)
