@@ -686,6 +686,7 @@ constexpr int kWholeValues = 40960, kWholeCtas = 2 * kSms;
 // measured on k_pages_tc: a CTA's start and end, a key tile of two row tiles, of one (the alternate walk), and
 // k_pages_rows' rate over own keys
 constexpr double kTcFixedUs = 8.0, kTcTileUs = 1.8, kTcAltTileUs = 1.0, kOwnBytesPerUs = 4.5e6;
+constexpr int kF32TcKeys = 4096, kF32RowsKeys = 4096;
 constexpr int kOwnCtas = 8 * kSms;           // k_pages_rows' CTAs over own keys: requests differ in length
 PagesPlan plan_attention(const PagesAttention &p) {
     PagesPlan pl{};
@@ -711,28 +712,31 @@ PagesPlan plan_attention(const PagesAttention &p) {
         pl.slots = 1;
         return pl;
     }
-    const auto splits = [&](long long ctas, long long want, long long keys) {   // key ranges that fill the GPU
-        return std::min<long long>({std::max<long long>(1, want / ctas), up(keys, kPagesOwnKeys), kPagesMaxSplits});
+    // key ranges that fill the GPU; fp32 queries: no longer than `most` (what the MMAs' accumulators cut off)
+    const auto splits = [&](long long ctas, long long want, long long keys, long long most) {
+        const long long least = f32 ? up(keys, most) : 1;
+        return std::min<long long>({std::max<long long>(least, want / ctas), up(keys, kPagesOwnKeys), kPagesMaxSplits});
     };
     if (bound > 0) {
         pl.own_tc = fits && own_rows > kTcMinOwnRows;
         pl.own_alt = pl.own_tc && (f32 || own_rows <= 128);
         pl.own_tiles = (int)up(own_rows, !pl.own_tc ? rt : pl.own_alt ? 128 : 256);
-        pl.own_splits = (int)splits((long long)ba.B * pl.own_tiles * nkv, pl.own_tc ? kSms : kOwnCtas, bound);
+        pl.own_splits = (int)splits((long long)ba.B * pl.own_tiles * nkv, pl.own_tc ? kSms : kOwnCtas, bound, pl.own_tc ? kF32TcKeys : kF32RowsKeys);
     }
     if (ba.prefix_len > 0) {
         pl.prefix_tc = fits && rows > kTcMinRows;
         pl.prefix_alt = pl.prefix_tc && (f32 || rows <= 128);
         pl.prefix_tiles = (int)up(rows, !pl.prefix_tc ? rt : pl.prefix_alt ? 128 : 256);
         const long long row_ctas = (long long)pl.prefix_tiles * nkv;
-        long long n = splits(row_ctas, pl.prefix_tc ? kSms : 2 * kSms, ba.prefix_len);
+        long long n = splits(row_ctas, pl.prefix_tc ? kSms : 2 * kSms, ba.prefix_len, pl.prefix_tc ? kF32TcKeys : kF32RowsKeys);
+        const long long least = f32 ? std::min<long long>(n, up(ba.prefix_len, kF32TcKeys)) : 1;
         if (pl.prefix_tc) {
             // k_pages_tc shares the GPU with the own keys' kernel: the fewest ranges that take no longer than
             // both kernels' work spread over all SMs (in us; own keys: half the tables' capacity)
             const double own_us = pl.own_tc ? 0.0 : 0.5 * (double)(ba.B * bound) * nkv * p.pg.hd * 4 * pl.own_tiles / kOwnBytesPerUs;
             const double tiles = (double)up(ba.prefix_len, 128), tile_us = pl.prefix_alt ? kTcAltTileUs : kTcTileUs;
             double best = 1e30;
-            for (long long k = n, most = n; k >= 1; --k) {
+            for (long long k = n, most = n; k >= least; --k) {
                 const double t = kTcFixedUs + std::ceil(tiles / k) * tile_us;
                 const double all = std::max(t, (double)(k * row_ctas) / kSms * t + own_us);
                 if (all <= best * (k == most ? 1.0 : 0.999)) {

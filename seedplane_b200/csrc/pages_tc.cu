@@ -14,7 +14,11 @@
 //   warp 9           issues the MMAs: while one row tile's scores are exponentiated, the other's products run
 // One row tile alone (at most 128 rows: a small batch, or fp32 queries) gives both groups of warps work by
 // taking alternate key tiles, each with its own (m, l, O); their partials are joined like those of key ranges.
-// fp32 queries: Q as fp16 hi and lo tiles, S = Qhi K^T + Qlo K^T, P as hi and lo, O += Phi V + Plo V.
+// fp32 queries: Q as fp16 hi and lo tiles, S = Qlo K^T + Qhi K^T, P as hi and lo, O += Plo V + Phi V. The MMAs cut off
+// what they add to an accumulator, 2^-24 of it an addition: the small products go first (S: 3.7e-6 -> 2.4e-6 of the
+// result after 32,768 keys), and every kTcFlush tiles O is added to a second set of columns with ordinary rounding
+// (3,100 keys at once: 8e-6; every 4 tiles 1.6e-6, every 2 1.1e-6). Two groups that share a row tile have no
+// columns to spare: their key ranges are kept short instead.
 // Slots of a page behind the last key may hold anything: their scores are replaced, their V rows zeroed in
 // shared memory (0 x NaN would reach O). Every wait is bounded.
 #include <cuda.h>
@@ -36,6 +40,7 @@ constexpr int kTcThreads = kTcSoftmax + 64;
 constexpr int kTcProducer = 16, kTcMma = 17; // warps
 constexpr int kTcStages = 4;
 constexpr uint32_t kTcSpin = 1u << 22;
+constexpr int kTcFlush = 2;                  // fp32 queries: O is added up in fp32 outside the MMAs every so many tiles
 constexpr float kTcGrow = 8.0f;              // log2 of the growth a running maximum may lag behind
 
 template <int HD>
@@ -69,15 +74,6 @@ SP_DEVINL void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
                  ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
                    "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]));
-}
-SP_DEVINL void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
-          "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
-          "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]));
 }
 // Two fp32 values as one 64-bit operand of the packed instructions.
 SP_DEVINL uint64_t f2(float a, float b) { return (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32); }
@@ -342,11 +338,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const uint64_t qd = smem_desc_sw128(base + (uint32_t)(kSplit || alt ? 0 : q) * L::kTile, 1024);
                 if (elect_one()) {
 #pragma unroll
-                    for (int part = 0; part < (kSplit ? 2 : 1); ++part)
+                    for (int part = kSplit ? 1 : 0; part >= 0; --part)    // the small products first
 #pragma unroll
                         for (int kk = 0; kk < KS; ++kk) {
                             const int o = ((kk >> 2) * L::kHalf + (kk & 3) * 32) >> 4;
-                            mma_f16_id(tmem + 128 * q, qd + o + ((part * L::kTile) >> 4), kd + o, id_s, part + kk > 0);
+                            mma_f16_id(tmem + 128 * q, qd + o + ((part * L::kTile) >> 4), kd + o, id_s, (kSplit && part == 0) || kk > 0);
                         }
                     mma_commit(&bar.s_full[q]);
                 }
@@ -359,11 +355,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 tc_fence_after();
                 if (elect_one()) {
 #pragma unroll
-                    for (int part = 0; part < (kSplit ? 2 : 1); ++part)
+                    for (int part = kSplit ? 1 : 0; part >= 0; --part)
 #pragma unroll
                         for (int kk = 0; kk < kTcKeys / 16; ++kk)
                             mma_ts(tmem + 256 + 128 * q, tmem + 128 * q + 32 * (kk >> 1) + 8 * (kk & 1) + 16 * part, vd + ((kk * 2048) >> 4), id_o,
-                                   !(first && part + kk == 0));
+                                   !(first && part == (kSplit ? 1 : 0) && kk == 0));
                 }
                 __syncwarp();
                 return true;
@@ -393,7 +389,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 for (int i = 0; i < n && ok; ++i) {
                     for (int q = 0; q < nq && ok; ++q) {
                         if (q == 0 && (!arrive(v_st) || (i + 1 < n && !arrive(k_st)))) break;
-                        if (!values(q, i == 0)) break;
+                        if (!values(q, i % (kSplit ? kTcFlush : INT_MAX) == 0)) break;
                         if (q == nq - 1) commit(&bar.empty[v_st]);
                         if (i + 1 < n) {
                             scores(q);
@@ -464,7 +460,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const float c = p.scale * 1.4426950408889634f;
             float m = -INFINITY, l = 0.f;
             uint32_t ph = 0u;
-            bool ok = true, any = false;
+            bool ok = true, any = false, flushed = false;
             // the two halves of a row's columns: their threads exchange a value through shared memory
             const auto swap = [&](float v) -> float {
                 s_swap[grp][half][r & 127] = v;
@@ -502,19 +498,31 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 const float mine = fmaxf(mx[0], mx[1]), mt = fmaxf(mine, swap(mine)) * c;
                 const bool grow = mt > m + kTcGrow || (!any && mt > m);
-                if (any && __any_sync(0xffffffffu, grow)) {
+                const bool flush = kSplit && !alt && i > 0 && i % kTcFlush == 0;
+                if (any && (flush || __any_sync(0xffffffffu, grow))) {
                     // s_full of this tile came after the products of the tile before: O is at rest
                     const float f = grow ? exp2_approx(m - mt) : 1.f;
                     l *= f;
-#pragma unroll
-                    for (int k = 0; k < HD / 64; ++k) {
-                        uint32_t o[32];
-                        tmem_ld32_nowait(to + HD / 2 * half + 32 * k, o);
+#pragma unroll 1
+                    for (int k = 0; k < HD / 32; ++k) {
+                        const uint32_t at = to + HD / 2 * half + 16 * k;
+                        uint32_t o[16], t[16];
+                        tmem_ld16_nowait(at, o);
+                        if (flushed) tmem_ld16_nowait(at + 128, t);
                         tmem_wait_ld();
+                        if (flush || flushed) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                        tmem_st32(to + HD / 2 * half + 32 * k, o);
+                            for (int j = 0; j < 16; ++j)
+                                t[j] = __float_as_uint(((flushed ? __uint_as_float(t[j]) : 0.f) + (flush ? __uint_as_float(o[j]) : 0.f)) * f);
+                            tmem_st16(at + 128, t);
+                        }
+                        if (!flush) {                        // else the tile's products start O anew
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                            tmem_st16(at, o);
+                        }
                     }
+                    flushed |= flush;
                 }
                 if (grow) m = mt;
                 any = true;
@@ -567,6 +575,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (any && ok) {
                     tmem_ld32_nowait(to + HALF * half + 32 * k, o);
                     tmem_wait_ld();
+                    if (flushed) {
+                        uint32_t t[32];
+                        tmem_ld32_nowait(to + 128 + HALF * half + 32 * k, t);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) + __uint_as_float(t[j]));
+                    }
                 } else {
 #pragma unroll
                     for (int j = 0; j < 32; ++j) o[j] = 0u;
