@@ -276,7 +276,7 @@ SP_DEVINL void ldsm4t(uint32_t addr, uint32_t &r0, uint32_t &r1, uint32_t &r2, u
 }
 
 template <int HD, typename TQ, typename TC>
-__global__ void __launch_bounds__(32 * kRowsWarps) k_pages_rows(PagesAttention p, PagesPlan pl) {
+__global__ void __launch_bounds__(32 * kRowsWarps, 3) k_pages_rows(PagesAttention p, PagesPlan pl) {
     constexpr bool kSplit = sizeof(TQ) == 4;                 // fp32 queries: hi / lo halves
     constexpr int RT = kSplit ? 8 : 16;                      // rows per CTA
     constexpr int KT = kRowsTileBytes / (HD * 2);            // keys per warp tile: 16 or 32

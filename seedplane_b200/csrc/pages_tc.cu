@@ -8,10 +8,14 @@
 //         and O seldom need rescaling (P <= 256 then, exact in either 16-bit type's range); written over
 //         S_q in TMEM in the cache's type
 //   O_q += P_q V     tcgen05.mma with A = P_q in TMEM, B = V as it lies in its pages (MN-major)
-// Bound by the exponentials (16 a clock and SM) and the MMAs, which take equally long for head_dim 128:
-//   warps 0-3, 4-7   one row tile each: thread = row. tcgen05.ld of 128 scores, maximum, exponentials, tcgen05.st
-//   warp 8           TMA of the pages' rows (64 dims x a page's slots a box, 128-byte swizzle) into a ring
-//   warp 9           issues the MMAs: while one row tile's scores are exponentiated, the other's products run
+// Packed prompts (12 requests, 3,552 rows x 28 heads over 3,001 + 560 keys) take 195 us, 917 TFLOP/s, at the 1,000 W
+// cap (1.8 GHz); the MMAs alone take 127 us, with the tiles' loads 151, the softmax with the loads 176. A row tile's
+// steps follow one another, so two row tiles take turns:
+//   warps 0-7, 8-15  one row tile each, two threads a row with 64 columns each: tcgen05.ld of the scores, maximum,
+//                    exponentials (in fp32, base 2), tcgen05.st in place (one thread a row and 128 registers of
+//                    scores was 5 % slower for decode steps, 2 % faster for prompts)
+//   warp 16          TMA of the pages' rows (64 dims x a page's slots a box, 128-byte swizzle) into a ring
+//   warp 17          issues the MMAs: while one row tile's scores are exponentiated, the other's products run
 // One row tile alone (at most 128 rows: a small batch, or fp32 queries) gives both groups of warps work by
 // taking alternate key tiles, each with its own (m, l, O); their partials are joined like those of key ranges.
 // fp32 queries: Q as fp16 hi and lo tiles, S = Qlo K^T + Qhi K^T, P as hi and lo, O += Plo V + Phi V. The MMAs cut off
@@ -232,10 +236,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_init(&bar.full[i], 1);
             mbar_init(&bar.empty[i], 1);
         }
-        mbar_init(&bar.q_full, kTcSoftmax);
+        mbar_init(&bar.q_full, kTcSoftmax / 32);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar.s_full[i], 1);
-            mbar_init(&bar.p_full[i], kTcSoftmax / 2);
+            mbar_init(&bar.p_full[i], kTcSoftmax / 64);
             mbar_init(&bar.o_full[i], 1);
         }
         mbar_init(&bar.tail, 1);
@@ -450,7 +454,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
         }
         fence_proxy_async_smem();
-        mbar_arrive(&bar.q_full);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.q_full);
         if (grp < nq) {
             const int r = (alt ? 0 : grp * kTcRows) + (warp & 3) * 32 + lane, row = row0 + r;
             const bool live = r < nrows;
@@ -553,7 +558,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 l += f2_lo(sum[0]) + f2_hi(sum[0]);
                 tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(&bar.p_full[grp]);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar.p_full[grp]);
                 // the next tile's swap writes what this one read: this tile's MMAs lie between (s_full)
             }
             // O and the row's statistics, half of the dims per thread. A warp's 32 half rows go through shared memory
