@@ -1845,7 +1845,7 @@ int check_pages(const sp_pages *pages, const sp_page_batch *batch, int32_t heads
     if (batch->tokens > 0 && (batch->batch < 1 || batch->max_q < 1 || !batch->lens_dev))
         return fail(SP_ERR_INVALID, "batch: %d rows of %d requests, max_q %d, %s", batch->tokens, batch->batch, batch->max_q,
                     batch->lens_dev ? "lens" : "no lens");
-    if (batch->table_width > 0 && (!batch->tables_dev || batch->table_stride < batch->table_width))
+    if (batch->batch > 0 && batch->table_width > 0 && (!batch->tables_dev || batch->table_stride < batch->table_width))
         return fail(SP_ERR_INVALID, "batch: %s, rows %lld apart for %d pages", batch->tables_dev ? "tables" : "no tables",
                     (long long)batch->table_stride, batch->table_width);
     if (batch->prefix_len > 0 && !batch->prefix_dev) return fail(SP_ERR_INVALID, "batch: prefix without pages");

@@ -778,10 +778,12 @@ cudaError_t attention_typed(const PagesAttention &p, PagesPlan pl, cudaStream_t 
             k_pages_rows<HD, TQ, TC><<<dim3(items, nkv), 32 * kRowsWarps, kRowsSmem, s>>>(p, pl);
     }
     if (e == cudaSuccess) e = cudaGetLastError();
-    if (e == cudaSuccess && pl.slots != 1)
+    if (e == cudaSuccess && pl.slots == 0)                   // no keys at all: zeros, and nothing to start beside
+        k_pages_merge<HD, TQ><<<(unsigned)(p.ba.T * p.nh), 32 * kMergeWarps, 0, s>>>(p, pl);
+    else if (e == cudaSuccess && pl.slots != 1)
         e = launch_dependent(k_pages_merge<HD, TQ>, dim3((unsigned)(p.ba.T * p.nh)),
                              32 * kMergeWarps, 0, s, p, pl);
-    return e;
+    return e != cudaSuccess ? e : cudaGetLastError();
 }
 
 }  // namespace

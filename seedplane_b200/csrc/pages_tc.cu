@@ -5,10 +5,10 @@
 // prefix, or the prefix and then one request's own keys) in tiles of 128 keys:
 //   S_q = Q_q K^T    tcgen05.mma M 128, N 128 into TMEM (two row tiles q, 128 columns each)
 //   P_q = 2^(S c - m), m the row's running maximum, kept while it grows by less than 2^8, so that the sums
-//         and O seldom need rescaling (P <= 256 then, exact in either 16-bit type's range); written over
+//         and O seldom need rescaling (P <= 256 then, within either 16-bit type's range); written over
 //         S_q in TMEM in the cache's type
 //   O_q += P_q V     tcgen05.mma with A = P_q in TMEM, B = V as it lies in its pages (MN-major)
-// Packed prompts (12 requests, 3,552 rows x 28 heads over 3,001 + 560 keys) take 195 us, 917 TFLOP/s, at the 1,000 W
+// Packed prompts (12 requests, 3,679 rows x 28 heads over 3,001 + 560 keys) take 195 us, 917 TFLOP/s, at the 1,000 W
 // cap (1.8 GHz); the MMAs alone take 127 us, with the tiles' loads 151, the softmax with the loads 176. A row tile's
 // steps follow one another, so two row tiles take turns:
 //   warps 0-7, 8-15  one row tile each, two threads a row with 64 columns each: tcgen05.ld of the scores, maximum,

@@ -247,6 +247,18 @@ def test_attention_of_large_scores_and_infinite_keys_out_of_sight():
     assert float((got.double() - ref).norm() / ref.norm()) < 0.02
 
 
+def test_attention_without_any_key_gives_zeros():
+    from seedplane_b200 import paged
+    pages = paged.PagedKV(1, 2, 64, 3, 16, device="cuda")
+    batch = paged.PageBatch(torch.zeros(2, 0, dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda"))
+    out, lse = torch.full((2, 4, 64), 7.0, device="cuda").half(), torch.full((2, 4), 7.0, device="cuda")
+    got = paged.attention(pages, 0, batch, torch.ones(2, 4, 64, device="cuda").half(), out=out, lse=lse)
+    pages.status()
+    assert (got == 0).all() and torch.isneginf(lse).all()
+    none = paged.PageBatch(torch.zeros(0, 1, dtype=torch.int32, device="cuda"), torch.zeros(0, dtype=torch.int32, device="cuda"))
+    assert paged.attention(pages, 0, none, torch.ones(0, 4, 64, device="cuda").half()).shape == (0, 4, 64)
+
+
 def test_attention_records_bad_tables_and_goes_on():
     from seedplane_b200 import paged
     from seedplane_b200._native import EngineError
