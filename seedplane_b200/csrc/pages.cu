@@ -611,8 +611,9 @@ __global__ void __launch_bounds__(32 * kMergeWarps) k_pages_merge(PagesAttention
     const PageBatchView &ba = p.ba;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int t = blockIdx.x / p.nh, h = blockIdx.x - t * p.nh;
-    if (t >= total_rows(ba)) return;
-    griddep_wait();
+    const bool none = t >= total_rows(ba);
+    griddep_wait();                                          // every CTA: the next grid in the stream starts after all of them
+    if (none) return;
     const long long step = (long long)ba.T * p.nh, at = blockIdx.x;
     float2 ml[NS];
     float M = -INFINITY, L = 0.f;
