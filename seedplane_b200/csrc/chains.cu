@@ -47,14 +47,17 @@ struct ChainStat {                           // of a chunk or a row
     int first;                               // first index of the maximum
     int pad_;
 };
+// T, the largest finite number for an infinite one: 0 x -inf would be NaN, and 1 / T = 0 means greedy
+SP_DEVINL float chain_t(const ChainArgs &a, int b) {
+    const float t = a.temperature ? a.temperature[b] : 1.f;
+    return t > FLT_MAX ? FLT_MAX : t;
+}
 SP_DEVINL float chain_k2(const ChainArgs &a, int b) {        // log2(e) / T; 0: greedy
-    if (!a.temperature) return 1.4426950408889634f;
-    const float t = a.temperature[b];
+    const float t = chain_t(a, b);
     return t > 0.f ? 1.4426950408889634f / t : 0.f;
 }
 SP_DEVINL double chain_inv_t(const ChainArgs &a, int b) {    // 0: greedy
-    if (!a.temperature) return 1.0;
-    const float t = a.temperature[b];
+    const float t = chain_t(a, b);
     return t > 0.f ? 1.0 / (double)t : 0.0;
 }
 // exp((l - m) / T), approximate: 1 at the maximum (also an infinite one), 0 for NaN and -inf

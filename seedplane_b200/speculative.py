@@ -284,7 +284,7 @@ def accept_chains(target_logits, draft_logits, drafts, u, *, counts=None, temper
         if draft_logits.shape != (B, n, V) or draft_logits.dtype != target_logits.dtype or draft_logits.device != dev or \
                 (n > 0 and draft_logits.stride(2) != 1):
             raise ValueError(f"draft_logits: [{B}, {n}, {V}] like target_logits expected")
-        draft, dbs, dld = draft_logits.data_ptr(), draft_logits.stride(0), draft_logits.stride(1)
+        draft, dbs, dld = draft_logits.data_ptr(), draft_logits.stride(0), draft_logits.stride(1) if n > 1 else V
 
     def need(t, name, want, shape):
         if t.dtype != want or t.device != dev or t.shape != shape or not t.is_contiguous():
@@ -309,7 +309,7 @@ def accept_chains(target_logits, draft_logits, drafts, u, *, counts=None, temper
         tokens_at = need(out[0], "out tokens", torch.int32, (B, n1))
         accepted_at = need(out[1], "out accepted", torch.int32, (B,))
     N.check(lib.sp_accept_chains(
-        dev.index, B, n, V, target_logits.data_ptr(), target_logits.stride(0), target_logits.stride(1), draft, dbs, dld, dtype,
+        dev.index, B, n, V, target_logits.data_ptr(), target_logits.stride(0), target_logits.stride(1) if n else V, draft, dbs, dld, dtype,
         drafts_at, counts_at, u_at, temperature_at, tokens_at, accepted_at, ws.data_ptr(), size, _raw_stream(dev.index)))
     return out
 

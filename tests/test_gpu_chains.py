@@ -82,6 +82,29 @@ def test_filtered_infinite_and_empty_rows():
     assert run(target, None, drafts, u) == oracle.chains(target, None, drafts, u, None, None)
 
 
+def test_infinite_temperature_is_the_flattest_and_tiny_ones_are_greedy():
+    """T = inf weighs every logit above -inf alike, as the largest finite T does; T = NaN is greedy; a T whose 1 / T
+    overflows leaves the maximum alone."""
+    target, draft, drafts, u = case(4, 3, 700, torch.float32, seed=31)
+    target[:, :, ::3] = -math.inf
+    t = torch.tensor([math.inf, math.inf, math.nan, 1e-42])
+    same = torch.tensor([torch.finfo(torch.float32).max] * 2 + [0.0, 0.0])
+    for d in (draft, None):
+        assert run(target, d, drafts, u, None, t) == oracle.chains(target, d, drafts, u, None, same)
+
+
+def test_single_rows_of_any_row_stride():
+    """A dimension of one row has no stride of its own."""
+    from seedplane_b200 import speculative
+    target, _, drafts, u = case(5, 0, 301, torch.float32, seed=33)
+    rows = target.cuda().as_strided((5, 1, 301), (301, 1, 1))
+    tokens, accepted = speculative.accept_chains(rows, None, drafts.cuda(), u.cuda())
+    assert (tokens.tolist(), accepted.tolist()) == oracle.chains(target, None, drafts, u, None, None)
+    target, draft, drafts, u = case(5, 1, 301, torch.float32, seed=34)
+    tokens, accepted = speculative.accept_chains(target.cuda(), draft.cuda().as_strided((5, 1, 301), (301, 5, 1)), drafts.cuda(), u.cuda())
+    assert (tokens.tolist(), accepted.tolist()) == oracle.chains(target, draft, drafts, u, None, None)
+
+
 def test_identical_distributions_accept_everything_and_extreme_numbers():
     target, _, drafts, u = case(3, 4, 777, torch.float32, seed=11)
     draft = target[:, :4].clone()
