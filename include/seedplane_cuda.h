@@ -305,7 +305,8 @@ int sp_pages_attention(int device, const sp_pages *pages, const sp_page_batch *b
  * kv_heads and head_dim (their status_dev is not used: sp_device_status reports). argmax_dev int32 [batch]:
  * the greedy token after each request's last row; logits_dev: NULL or fp32 [batch][vocab]. Every request
  * has at least one row; batch 1 .. 256, tokens 1 .. 512 (and exactly q_start[batch]). Like sp_prefill_batch
- * and sp_decode_batch, for caches that share a prefix. The engine's workspace is used. */
+ * and sp_decode_batch, for caches that share a prefix. The engine's workspace is used, and grows with the
+ * passes: a stream that is being captured is refused. */
 int sp_forward_pages(sp_engine *e, const sp_pages *layer_pages, const sp_page_batch *batch, const int32_t *tokens_dev,
                      float *logits_dev, int32_t *argmax_dev, void *stream);
 
@@ -328,7 +329,7 @@ int64_t sp_accept_chains_workspace(int32_t batch, int32_t drafts, int32_t vocab)
  * certain, q_i = 1 at its token), draft i is accepted when u[b][i] * q_i(x_i) < p_i(x_i). After the
  * first refusal i the next token is drawn from max(p_i - q_i, 0), or from p_i where that is zero
  * everywhere; after n acceptances from p_n. A draw from weights r is the first index whose running
- * sum exceeds u[b][drafts] * (their sum). T_b = temperature_dev[b] (fp32; NULL: 1); T_b <= 0: greedy,
+ * sum exceeds u[b][drafts] * (their sum). T_b = temperature_dev[b] (fp32; NULL: 1); T_b <= 0 or NaN: greedy,
  * p_i is 1 at the row's first maximum. NaN logits weigh nothing; a row without a finite or +inf logit
  * accepts nothing and draws -1; a drafted token outside [0, vocab) is refused.
  * target_dev: [b][drafts + 1][vocab], rows target_ld and requests target_bs elements apart; draft_dev:

@@ -1949,7 +1949,7 @@ int sp_pages_attention(int device, const sp_pages *pages, const sp_page_batch *b
 
 // What the paged passes have in common: the checks, and the layers' parameter blocks without their pages.
 static int paged_pass_args(sp_engine *e, const sp_pages *layer_pages, const sp_page_batch *batch, PagesAppend &ap,
-                           PagesAttention &at) {
+                           PagesAttention &at, cudaStream_t s) {
     if (!e || !layer_pages || !batch) return fail(SP_ERR_INVALID, "null argument");
     if (!e->prefill) return fail(SP_ERR_UNSUPPORTED, "paged passes need the batched pass (SEEDPLANE_PREFILL=steps)");
     const sp_config &c = e->c;
@@ -1977,6 +1977,10 @@ static int paged_pass_args(sp_engine *e, const sp_pages *layer_pages, const sp_p
     ap.ba = at.ba;
     at.scale = 1.0f / sqrtf((float)c.head_dim);
     SP_CUDA(cudaSetDevice(e->device));
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    SP_CUDA(cudaStreamIsCapturing(s, &cap));
+    if (cap != cudaStreamCaptureStatusNone)                  // a later, larger pass may move the workspace a graph would keep
+        return fail(SP_ERR_UNSUPPORTED, "paged passes cannot be captured into a graph");
     size_t need = 0;
     for (int l = 0; l < c.layers; ++l) {                     // the plan depends on the pages' layout
         int rc = attention_args(&layer_pages[l], batch, c.heads, SP_F32, at);
@@ -2027,7 +2031,7 @@ int sp_forward_pages(sp_engine *e, const sp_pages *layer_pages, const sp_page_ba
     PagesAppend ap{};
     PagesAttention at{};
     if (!tokens_dev || !argmax_dev) return fail(SP_ERR_INVALID, "null argument");
-    int rc = paged_pass_args(e, layer_pages, batch, ap, at);
+    int rc = paged_pass_args(e, layer_pages, batch, ap, at, (cudaStream_t)stream);
     if (rc) return rc;
     return paged_pass(e, layer_pages, batch, ap, at, tokens_dev, logits_dev, argmax_dev, (cudaStream_t)stream);
 }
@@ -2040,7 +2044,7 @@ int sp_decode_pages(sp_engine *e, const sp_pages *layer_pages, const sp_page_bat
     if (n_steps <= 0) return fail(SP_ERR_INVALID, "n_steps must be positive");
     if (batch && (batch->q_start_dev || batch->max_q != 1 || batch->tokens != batch->batch || batch->batch > kBatchMax))
         return fail(SP_ERR_INVALID, "a decode batch has one row per request, no q_start, at most %d requests", kBatchMax);
-    int rc = paged_pass_args(e, layer_pages, batch, ap, at);
+    int rc = paged_pass_args(e, layer_pages, batch, ap, at, (cudaStream_t)stream);
     if (rc) return rc;
     cudaStream_t s = (cudaStream_t)stream;
     if (!e->bt) SP_CUDA(cudaMalloc(&e->bt, sizeof(BatchIn)));

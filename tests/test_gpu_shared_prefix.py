@@ -143,3 +143,23 @@ def test_grouped_lease_with_a_prefix(tiny):
     assert plain == shared
     with pytest.raises(ValueError):
         ex({"prefix_ids": head, "batch": [{"ids": tails[0], "max_new_tokens": 60}]})
+
+
+def test_passes_are_not_captured(tiny):
+    """The engine may move its workspace for a later, larger pass: a graph must not keep it."""
+    from seedplane_b200.paged import PageBatch
+    eng, cfg, _ = tiny
+    dev = eng.device
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    pages = eng.new_pages(4, 64)
+    batch, tokens = PageBatch(i32([[0], [1]]), i32([1, 1])), i32([3, 4])
+    want = eng.forward_pages(pages, batch, tokens)[0].tolist()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        for call in (lambda: eng.forward_pages(pages, batch, tokens), lambda: eng.decode_pages(pages, batch, tokens, 2)):
+            with pytest.raises(RuntimeError, match="captured"):
+                call()
+    assert eng.forward_pages(pages, batch, tokens)[0].tolist() == want
+    eng.status()
