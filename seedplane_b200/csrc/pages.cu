@@ -603,6 +603,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 3) k_pages_rows(PagesAttentio
 // way; a slot without weight (a range that does not exist) is passed over. The warps' sums are added in order.
 constexpr int kMergeWarps = 4;
 constexpr int kMergeSlots = 4 * kPagesMaxSplits;
+constexpr int kMergeFew = 32, kMergeFewCtas = 148 * 16;
 template <int HD, typename TQ>
 __global__ void __launch_bounds__(32 * kMergeWarps) k_pages_merge(PagesAttention p, PagesPlan pl) {
     constexpr int DL = HD / 32, NS = kMergeSlots / 32, BATCH = 8;
@@ -678,15 +679,87 @@ __global__ void __launch_bounds__(32 * kMergeWarps) k_pages_merge(PagesAttention
     if (p.lse && threadIdx.x == 0) p.lse[at] = row_lse(M, L);
 }
 
-// Which kernel takes what. k_pages_tc pads a row tile to 128 rows and needs an SM to itself;
-// k_pages_rows reads K and V again for every 16 rows (8 with fp32 queries).
+// The same with a warp per (token, head), for at most 32 ranges: no shared memory, no barrier. Where a CTA per (token,
+// head) no longer has them all on the GPU at once: with their attention, 3,976 (token, heads)
+// of 11 ranges 50.2 -> 46.1 us, 22,400 of 2 118 -> 96; but 1,792 of 20 39.1 -> 39.9.
+template <int HD, typename TQ>
+__global__ void __launch_bounds__(32 * kMergeWarps) k_pages_merge_few(PagesAttention p, PagesPlan pl) {
+    constexpr int DL = HD / 32, BATCH = 8;
+    const PageBatchView &ba = p.ba;
+    const int lane = threadIdx.x & 31;
+    const long long step = (long long)ba.T * p.nh, at = (long long)blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
+    const int t = (int)(at / p.nh), h = (int)(at - (long long)t * p.nh);
+    const bool none = t >= total_rows(ba);
+    griddep_wait();
+    if (none) return;
+    const float2 ml = lane < pl.slots ? *reinterpret_cast<const float2 *>(pl.ml + (lane * step + at) * 2) : make_float2(-INFINITY, 0.f);
+    const float M = warp_max(ml.x), w = exp2_approx(ml.x - (M == -INFINITY ? 0.f : M)), L = warp_sum(ml.y * w);
+    float acc[DL];
+#pragma unroll
+    for (int d = 0; d < DL; ++d) acc[d] = 0.f;
+    for (int s0 = 0; s0 < pl.slots; s0 += BATCH) {
+        float f[BATCH], v[BATCH][DL];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            f[i] = __shfl_sync(0xffffffffu, w, s0 + i);          // 0 behind the last
+#pragma unroll
+            for (int d = 0; d < DL; ++d) v[i][d] = 0.f;
+            if (!(f[i] == 0.f)) {
+                const float *src = pl.acc + ((s0 + i) * step + at) * HD + lane * DL;
+                if constexpr (DL == 4) {
+                    const float4 x = *reinterpret_cast<const float4 *>(src);
+                    v[i][0] = x.x;
+                    v[i][1] = x.y;
+                    v[i][2] = x.z;
+                    v[i][3] = x.w;
+                } else {
+                    const float2 x = *reinterpret_cast<const float2 *>(src);
+                    v[i][0] = x.x;
+                    v[i][1] = x.y;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i)
+#pragma unroll
+            for (int d = 0; d < DL; ++d) acc[d] = fmaf(v[i][d], f[i], acc[d]);
+    }
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    TQ *dst = reinterpret_cast<TQ *>(p.out) + (long long)t * p.out_stride + h * HD + lane * DL;
+#pragma unroll
+    for (int d = 0; d < DL; ++d) acc[d] = L == L ? acc[d] * inv : L;
+    if constexpr (sizeof(TQ) == 4) {
+        if constexpr (DL == 4) *reinterpret_cast<float4 *>(dst) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        else *reinterpret_cast<float2 *>(dst) = make_float2(acc[0], acc[1]);
+    } else {
+        if constexpr (DL == 4) *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2<TQ>(acc[0], acc[1]), pack2<TQ>(acc[2], acc[3]));
+        else *reinterpret_cast<uint32_t *>(dst) = pack2<TQ>(acc[0], acc[1]);
+    }
+    if (p.lse && lane == 0) p.lse[at] = row_lse(M, L);
+}
+
+// Which kernel takes what. k_pages_tc pads a row tile to 128 rows and needs an SM to itself; k_pages_rows reads K and
+// V again for every 16 rows (8 with fp32 queries).
 constexpr int kSms = 148;
+// The prefix: up to 32 rows a kv head by k_pages_rows (28 rows of 4 heads over 4,096 keys 13.0 against 14.6 us, over
+// 16,384 20.5 against 21.2), more by k_pages_tc once the reads beyond those of 32 rows pass so many bytes (35 rows over
+// 4,096 keys, 8 MB: 13.4 against 14.6; over 16,384, 34 MB: 28.8 against 21.3; fp32, 25 MB: 15.7 against 18.3, 34 MB:
+// 33.3 against 29.2).
 constexpr int kTcMinRows = 32;
+constexpr double kRowsReads = 12e6, kF32RowsReads = 28e6;
+// A request's own keys: by k_pages_tc from more rows than this on (8 requests of 84 rows 31.0 against 35.5 us, of 42
+// 24.2 against 23.8; fp32, of 126 47.4 against 49.7, of 63 37.2 against 31.4).
 constexpr int kTcMinOwnRows = 64;
 constexpr int kWholeValues = 40960, kWholeCtas = 2 * kSms;
 // measured on k_pages_tc: a CTA's start and end, a key tile of two row tiles, of one (the alternate walk), and
 // k_pages_rows' rate over own keys
 constexpr double kTcFixedUs = 8.0, kTcTileUs = 1.8, kTcAltTileUs = 1.0, kOwnBytesPerUs = 4.5e6;
+// Many rows a request: one walk over the prefix and the own keys, or parts that are joined. Fitted to 49 sizes (rows
+// 420 to 11,200, prefixes of 60 to 4,000 keys; the times within 5 and 8 %): a walk's start and end and its key tile,
+// as many rounds of them as the SMs need; the parts' start and join, a key tile's share of all SMs, the partials'
+// rate. 8 requests of 100 tokens, 4,000 keys: 80 us in one walk, 96 in parts; 4 requests: 79 and 59.
+constexpr double kWalkFixedUs = 13.0, kWalkTileUs = 2.0, kF32WalkTileUs = 3.0, kPartsFixedUs = 14.0, kPartsTileUs = 2.8,
+                 kJoinBytesPerUs = 3e6;
 constexpr int kF32TcKeys = 4096, kF32RowsKeys = 4096;
 constexpr int kOwnCtas = 8 * kSms;           // k_pages_rows' CTAs over own keys: requests differ in length
 PagesPlan plan_attention(const PagesAttention &p) {
@@ -698,12 +771,6 @@ PagesPlan plan_attention(const PagesAttention &p) {
     const long long rows = (long long)ba.T * G, own_rows = (long long)std::min(ba.max_q, ba.T) * G;
     const long long bound = (long long)ba.table_width * p.pg.page_size;
     const int pair = f32 ? 128 : 256;                        // rows of a k_pages_tc CTA that needs no partner
-    if (fits && bound > 0 && own_rows > 128 && rows * nkv / pair >= 96) {
-        pl.whole = pl.own_tc = 1;
-        pl.own_tiles = (int)up(own_rows, pair);
-        pl.slots = 1;
-        return pl;
-    }
     // few requests and a walk of at most 5 tiles a warp: one launch and no join (4 requests, 602 keys of 64
     // dims: 8.0 us on the GPU against 6.9 in two launches, but 10.2 a call in a loop against 13.0)
     const long long small_tiles = up(own_rows, rt);
@@ -725,7 +792,8 @@ PagesPlan plan_attention(const PagesAttention &p) {
         pl.own_splits = (int)splits((long long)ba.B * pl.own_tiles * nkv, pl.own_tc ? kSms : kOwnCtas, bound, pl.own_tc ? kF32TcKeys : kF32RowsKeys);
     }
     if (ba.prefix_len > 0) {
-        pl.prefix_tc = fits && rows > kTcMinRows;
+        const double read = (double)ba.prefix_len * nkv * p.pg.hd * 4;
+        pl.prefix_tc = fits && rows > kTcMinRows && (pl.own_tc || (up(rows, rt) - kTcMinRows / rt) * read > (f32 ? kF32RowsReads : kRowsReads));
         pl.prefix_alt = pl.prefix_tc && (f32 || rows <= 128);
         pl.prefix_tiles = (int)up(rows, !pl.prefix_tc ? rt : pl.prefix_alt ? 128 : 256);
         const long long row_ctas = (long long)pl.prefix_tiles * nkv;
@@ -751,6 +819,21 @@ PagesPlan plan_attention(const PagesAttention &p) {
         pl.prefix_slots = pl.prefix_splits << pl.prefix_alt;
     }
     pl.slots = pl.prefix_slots + (pl.own_splits << pl.own_alt);
+    // many rows a request: the prefix and the own keys in one walk, no partials
+    if (fits && bound > 0 && own_rows > 128) {
+        const long long tiles = up(own_rows, pair), items = std::min<long long>(ba.B * tiles, up(rows, pair) + ba.B / 2) * nkv;
+        const double prefix = (double)up(ba.prefix_len, 128), own = 0.5 * (double)up(bound, 128);
+        const double scale = f32 && p.pg.hd == 64 ? 0.7 : 1.0;
+        const double one = up(items, kSms) * (kWalkFixedUs + (prefix + own) * (f32 ? kF32WalkTileUs : kWalkTileUs) * scale);
+        const double parts = kPartsFixedUs + ((double)(up(rows, pair) * nkv) * prefix + items * own) * kPartsTileUs * scale / kSms +
+                             (double)ba.T * p.nh * p.pg.hd * 8 * pl.slots / kJoinBytesPerUs;
+        if (one <= parts) {
+            pl = PagesPlan{};
+            pl.whole = pl.own_tc = 1;
+            pl.own_tiles = (int)tiles;
+            pl.slots = 1;
+        }
+    }
     return pl;
 }
 size_t plan_bytes(const PagesAttention &p, const PagesPlan &pl) {
@@ -781,6 +864,9 @@ cudaError_t attention_typed(const PagesAttention &p, PagesPlan pl, cudaStream_t 
     if (e == cudaSuccess) e = cudaGetLastError();
     if (e == cudaSuccess && pl.slots == 0)                   // no keys at all: zeros, and nothing to start beside
         k_pages_merge<HD, TQ><<<(unsigned)(p.ba.T * p.nh), 32 * kMergeWarps, 0, s>>>(p, pl);
+    else if (e == cudaSuccess && pl.slots > 1 && pl.slots <= kMergeFew && p.ba.T * p.nh > kMergeFewCtas)
+        e = launch_dependent(k_pages_merge_few<HD, TQ>, dim3((unsigned)((p.ba.T * p.nh + kMergeWarps - 1) / kMergeWarps)),
+                             32 * kMergeWarps, 0, s, p, pl);
     else if (e == cudaSuccess && pl.slots != 1)
         e = launch_dependent(k_pages_merge<HD, TQ>, dim3((unsigned)(p.ba.T * p.nh)),
                              32 * kMergeWarps, 0, s, p, pl);
