@@ -196,6 +196,28 @@ def test_attention_of_short_prefixes_under_many_rows(prefix, dt, cache):
         check_attention(s, x, got)
 
 
+@pytest.mark.parametrize("dt,cache", [(F16, F16), (BF16, BF16), (F32, F16)])
+@pytest.mark.parametrize("prefix", [64, 127, 129, 300])
+def test_attention_of_hundreds_of_requests(prefix, dt, cache):
+    """Enough rows for the tensor-core walk of a short prefix, and for the join of a row by one warp."""
+    for batch, nh, nkv, hd, page in ((420, 14, 2, 64, 16), (200, 28, 4, 128, 32)):
+        s = oracle.make_batch(q=[1] * batch, lens=[(5 * i) % 41 for i in range(1, batch + 1)], prefix=prefix, page=page, nkv=nkv,
+                              hd=hd, dtype=cache, seed=prefix)
+        lse = torch.empty(s["rows"], nh, device="cuda")
+        x, got = run_attention(s, nh, dt, lse=lse)
+        check_attention(s, x, got, lse)
+
+
+@pytest.mark.parametrize("dt,cache", [(F16, F16), (BF16, BF16), (F32, F16)])
+@pytest.mark.parametrize("prefix", [1800, 1919, 2049, 6001])
+def test_attention_of_a_long_prefix_under_one_row_tile(prefix, dt, cache):
+    for page in (8, 256):
+        s = oracle.make_batch(q=[1] * 14, lens=[1 + 9 * i for i in range(14)], prefix=prefix, page=page, nkv=4, hd=128, dtype=cache,
+                              seed=prefix)
+        x, got = run_attention(s, 28, dt)
+        check_attention(s, x, got)
+
+
 @pytest.mark.parametrize("dt,cache,nh,nkv,hd", [(F16, F16, 28, 4, 128), (BF16, BF16, 14, 2, 64), (F32, F16, 12, 2, 128),
                                                 (F32, F16, 16, 8, 64)])
 @pytest.mark.parametrize("prefix,page", [(130, 64), (0, 16), (31, 128)])
