@@ -10,11 +10,13 @@
 //   k_chain_sums    (request, piece of the vocabulary): joins the chunks and walks the chain (every piece's CTA for
 //                   itself: less than a launch), then fp64 sums of the rows that are drawn from. The rows' fp32
 //                   sums decide a draft when u q and p differ by more than the sums may be off (kChainSlack); a
-//                   draft that is nearer (one in 10,000) leaves the request to the slow walk in k_chain_pick. A draw
+//                   draft that is nearer (one in 10,000) is summed as if refused and left to k_chain_pick. A draw
 //                   compares a running sum over the vocabulary with a given number, and an fp32 sum of 1e5 terms
 //                   would move the border by more than many tokens' whole probability.
 //   k_chain_left    (request, piece): fp64 sums of max(p - q, 0), for requests with a refused draft and a drafter
 //   k_chain_pick    a CTA per request: the piece and in it the index whose running sum passes u times the total
+// For 32 requests' five drafts, 152,064 logits, each alone and cold: 36, 26, 19 and 12 us; together 76, at a floor of
+// 32.7 (0.214 GB once, 6.5 TB/s). k_chain_stats runs at 5.9 TB/s; the others are short and wait for one another.
 // The pieces spread the requests' fp64 work (four exponentials a token after a refusal, else one) over all SMs; a
 // cluster of 8 CTAs per request for the last four took 43 us for 32 requests and 36 for 48 without a drafter, these
 // 40 and 24.
@@ -194,16 +196,16 @@ struct Weigh {                               // exp((l - max) / T) of a row's lo
 };
 
 // ---- the draw ----------------------------------------------------------------------------------
-enum ChainMode : int { CM_DONE = 0, CM_P = 1, CM_P_LESS = 2, CM_BOTH = 3, CM_SLOW = 4 };
+enum ChainMode : int { CM_DONE = 0, CM_P = 1, CM_P_LESS = 2, CM_BOTH = 3, CM_NEAR = 4, CM_SLOW = 5 };
 struct ChainPlan {                           // of a request, by chain_decide
     int mode;                                // weights: none (the token is written), p, p without the refused token,
-                                             // max(p - q, 0); or the slow walk
+                                             // max(p - q, 0); draft acc is too near to say; or two are (the slow walk)
     int acc;                                 // accepted drafts: the row that is drawn from
     float mp, mq;                            // the rows' maxima
 };
 struct ChainScratch {
     ChainStat *st;                           // [B][rows][chunks]
-    ChainPlan *plan;                         // [B]
+    ChainPlan *plan;                         // [B][2]: the plan; where a draft is too near, the one if it is accepted
     double *sp, *sq, *left;                  // [B][pieces]
     int piece, pieces;                       // logits of a piece, pieces of a row
     int chunk, chunks;                       // likewise of the statistics
@@ -214,9 +216,12 @@ inline int chain_piece(int B, int V) {
     return (long long)B * ((V + kPieceMost - 1) / kPieceMost) < 2 * 148 ? kPieceMost / 2 : kPieceMost;
 }
 
+SP_DEVINL Weigh chain_weigh_of(const ChainArgs &a, int b, const double *tab) {
+    return Weigh{tab, chain_inv_t(a, b) * 92.33248261689365807103517958412109, chain_k2(a, b)};
+}
 SP_DEVINL Weigh chain_weigh(const ChainArgs &a, int b, double *tab) {
     if (threadIdx.x < 64) tab[threadIdx.x] = c_exp_tab[threadIdx.x];
-    return Weigh{tab, chain_inv_t(a, b) * 92.33248261689365807103517958412109, chain_k2(a, b)};
+    return chain_weigh_of(a, b, tab);
 }
 // sums of a CTA, the same bits in every thread
 template <int THREADS>
@@ -301,31 +306,40 @@ SP_DEVINL ChainPlan chain_decide(const ChainArgs &a, const ChainScratch &sc, int
         s_dec[tid] = dec;
     }
     __syncthreads();
-    int acc = 0;
-    while (acc < cnt && s_dec[acc] == 1) ++acc;
-    const bool refused = acc < cnt;
-    ChainPlan plan{CM_DONE, acc, s_row[acc].max, refused && a.draft ? s_row[a.n + 1 + acc].max : -INFINITY};
     int pick = -1;
-    if (refused && s_dec[acc] == 2) plan.mode = CM_SLOW;
-    else if (plan.mp == -INFINITY) pick = -1;
-    else if (inv_t == 0.0) pick = s_row[acc].first;
-    else if (!refused || (a.draft && plan.mq == -INFINITY)) plan.mode = CM_P;    // a drafter's empty row takes nothing away
-    else plan.mode = a.draft ? CM_BOTH : CM_P_LESS;
-    if (write && tid == 0) sc.plan[b] = plan;
-    if (write && plan.mode != CM_SLOW) {
+    const auto walk = [&](int acc) {                         // on from draft acc
+        while (acc < cnt && s_dec[acc] == 1) ++acc;
+        const bool refused = acc < cnt;
+        ChainPlan plan{CM_DONE, acc, s_row[acc].max, refused && a.draft ? s_row[a.n + 1 + acc].max : -INFINITY};
+        pick = -1;
+        if (refused && s_dec[acc] == 2) plan.mode = CM_NEAR;
+        else if (plan.mp == -INFINITY) pick = -1;
+        else if (inv_t == 0.0) pick = s_row[acc].first;
+        else if (!refused || (a.draft && plan.mq == -INFINITY)) plan.mode = CM_P;    // a drafter's empty row takes nothing away
+        else plan.mode = a.draft ? CM_BOTH : CM_P_LESS;
+        return plan;
+    };
+    ChainPlan plan = walk(0);
+    if (plan.mode == CM_NEAR) {
+        const ChainPlan other = walk(plan.acc + 1);
+        if (other.mode == CM_NEAR) plan.mode = CM_SLOW;
+        if (write && tid == 0) sc.plan[2 * b + 1] = other;
+    }
+    if (write && tid == 0) sc.plan[2 * b] = plan;
+    if (write && plan.mode < CM_NEAR) {
         int *out = a.out_tokens + (size_t)b * (a.n + 1);
         for (int i = tid; i <= a.n; i += kPieceThreads)
-            if (i != acc) out[i] = i < acc ? tokens[i] : -1;
+            if (i != plan.acc) out[i] = i < plan.acc ? tokens[i] : -1;
             else if (plan.mode == CM_DONE) out[i] = pick;
-        if (tid == 0) a.accepted[b] = acc;
+        if (tid == 0) a.accepted[b] = plan.acc;
     }
     return plan;
 }
 
-// f(index, logits) of a piece [lo, hi) of row pr and, if given, qr
+// f(index, logits) of a piece [lo, hi) of row pr and, if given, qr, by THREADS threads
 template <typename T, int THREADS, typename F>
 SP_DEVINL void walk_piece(const T *pr, const T *qr, int lo, int hi, F f) {
-    for (int j0 = lo + threadIdx.x; j0 < hi; j0 += THREADS * kBatch) {
+    for (int j0 = lo + threadIdx.x % THREADS; j0 < hi; j0 += THREADS * kBatch) {
         float x[kBatch], y[kBatch];
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
@@ -350,8 +364,9 @@ __global__ void __launch_bounds__(kPieceThreads) k_chain_sums(ChainArgs a, Chain
     const int pieces = sc.pieces, b = blockIdx.x / pieces, k = blockIdx.x - b * pieces;
     const Weigh weigh = chain_weigh(a, b, s_tab);
     __syncthreads();
-    const ChainPlan plan = chain_decide<T>(a, sc, b, weigh, s_decide, k == 0);
+    ChainPlan plan = chain_decide<T>(a, sc, b, weigh, s_decide, k == 0);
     if (plan.mode == CM_DONE || plan.mode == CM_SLOW) return;
+    if (plan.mode == CM_NEAR) plan.mode = a.draft ? CM_BOTH : CM_P_LESS;     // as if it were refused
     const int lo = k * sc.piece, hi = min(a.V, lo + sc.piece);
     const T *pr = chain_row<T>(a, b, plan.acc);
     double sp = 0.0, sq = 0.0;
@@ -394,8 +409,8 @@ __global__ void __launch_bounds__(kPieceThreads) k_chain_left(ChainArgs a, Chain
     const Weigh weigh = chain_weigh(a, b, s_tab);
     __syncthreads();
     griddep_wait();
-    const ChainPlan plan = sc.plan[b];
-    if (plan.mode != CM_BOTH) return;
+    const ChainPlan plan = sc.plan[2 * b];
+    if (plan.mode != CM_BOTH && plan.mode != CM_NEAR) return;
     double sp, sq;
     piece_totals(sc.sp + (size_t)b * pieces, sc.sq + (size_t)b * pieces, pieces, sp, sq);
     const double ip = 1.0 / sp, iq = 1.0 / sq;
@@ -407,24 +422,18 @@ __global__ void __launch_bounds__(kPieceThreads) k_chain_left(ChainArgs a, Chain
     if (threadIdx.x == 0) sc.left[blockIdx.x] = sum;
 }
 
+// A request with a draft that is too near to say, by k_chain_pick's CTA: that draft, the tokens and the sums of the rows
+// that are drawn from. Not inlined: one request in some hundreds comes here (3 to 70 us more), and its code in line cost every
+// call 3 us.
 template <typename T>
-__global__ void __launch_bounds__(kPickThreads) k_chain_pick(ChainArgs a, ChainScratch sc) {
-    __shared__ double s_tab[64], s_sum[2][kPickThreads / 32];
-    __shared__ int s_pick, s_last;
-    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int pieces = sc.pieces;
-    const Weigh weigh = chain_weigh(a, b, s_tab);
+__device__ __noinline__ ChainPlan settle_near(const ChainArgs &a, const ChainScratch &sc, int b, const double *tab,
+                                              double (*s_sum)[kPickThreads / 32]) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, pieces = sc.pieces;
+    const Weigh weigh = chain_weigh_of(a, b, tab);
     const double *u = a.u + (size_t)b * (a.n + 1);
     const int *tokens = a.tokens + (size_t)b * a.n;
-    if (tid == 0) {
-        s_pick = INT_MAX;
-        s_last = -1;
-    }
-    __syncthreads();
-    griddep_wait();
-    ChainPlan plan = sc.plan[b];
-    if (plan.mode == CM_DONE) return;
     double *sp = sc.sp + (size_t)b * pieces, *sq = sc.sq + (size_t)b * pieces, *left = sc.left + (size_t)b * pieces;
+    ChainPlan plan = sc.plan[2 * b];
     const auto maximum = [&](const T *row) {                 // NaN ignored, the same in every thread
         float m = -INFINITY;
         for (int j = tid; j < a.V; j += kPickThreads) m = fmaxf(m, to_float(row[j]));
@@ -436,12 +445,11 @@ __global__ void __launch_bounds__(kPickThreads) k_chain_pick(ChainArgs a, ChainS
         for (int w = 1; w < kPickThreads / 32; ++w) d = fmax(d, s_sum[0][w]);
         return (float)d;
     };
-    // the pieces' sums by this CTA alone: fp(logit p), fq(logit q) into sp, sq, or one function into left
+    // the pieces' sums by this CTA alone, a warp a piece: of p and q into sp and sq, or of max(p - q, 0) into left
     const auto sums_here = [&](const T *pr, const T *qr, bool residual, double ip, double iq, double &tx, double &ty) {
-        tx = ty = 0.0;
-        for (int k = 0; k < pieces; ++k) {
+        for (int k = warp; k < pieces; k += kPickThreads / 32) {
             double x = 0.0, y = 0.0;
-            walk_piece<T, kPickThreads>(pr, qr, k * sc.piece, min(a.V, (k + 1) * sc.piece), [&](int, float lp, float lq) {
+            walk_piece<T, 32>(pr, qr, k * sc.piece, min(a.V, (k + 1) * sc.piece), [&](int, float lp, float lq) {
                 const double ep = weigh(lp, plan.mp), eq = weigh(lq, plan.mq);
                 if (residual) {
                     x += left_of(ep, ip, eq, iq);
@@ -450,16 +458,57 @@ __global__ void __launch_bounds__(kPickThreads) k_chain_pick(ChainArgs a, ChainS
                     y += eq;
                 }
             });
-            cta_sums<kPickThreads>(x, y, s_sum);
-            if (tid == 0) {
+            for (int o = 16; o > 0; o >>= 1) {
+                x += __shfl_xor_sync(0xffffffffu, x, o);
+                y += __shfl_xor_sync(0xffffffffu, y, o);
+            }
+            if (lane == 0) {
                 (residual ? left : sp)[k] = x;
                 if (!residual) sq[k] = y;
             }
-            tx += x;
-            ty += y;
         }
         __syncthreads();
+        piece_totals(residual ? left : sp, residual ? left : sq, pieces, tx, ty);
+        __syncthreads();                                     // read before the next sums
     };
+    // what chain_decide left open
+    const auto write = [&] {
+        int *out = a.out_tokens + (size_t)b * (a.n + 1);
+        for (int i = tid; i <= a.n; i += kPickThreads) out[i] = i < plan.acc ? tokens[i] : -1;
+        if (tid == 0) a.accepted[b] = plan.acc;
+        __syncthreads();                                     // the drawn token comes on top
+    };
+    const auto take_out = [&](const T *pr, int x) {          // the refused token out of its piece
+        if (x < 0 || x >= a.V) return;
+        const int k = x / sc.piece;
+        double y = 0.0, none = 0.0;
+        walk_piece<T, kPickThreads>(pr, (const T *)nullptr, k * sc.piece, min(a.V, (k + 1) * sc.piece),
+                                    [&](int j, float l, float) { y += weigh(j == x ? -INFINITY : l, plan.mp); });
+        cta_sums<kPickThreads>(y, none, s_sum);
+        if (tid == 0) sp[k] = y;
+        __syncthreads();
+    };
+    if (plan.mode == CM_NEAR) {
+        // the near draft in 64 bits, by the sums that its refusal needs (without a drafter: of p without it)
+        double tp, tq, qx = 1.0;
+        piece_totals(sp, sq, pieces, tp, tq);
+        const int x = tokens[plan.acc];
+        const double wp = weigh(to_float(chain_row<T>(a, b, plan.acc)[x]), plan.mp);
+        if (a.draft) qx = weigh(to_float(chain_row<T>(a, b, a.n + 1 + plan.acc)[x]), plan.mq) / tq;
+        else tp += wp;
+        const bool accepted = u[plan.acc] * qx < wp / tp;
+        if (accepted) plan = sc.plan[2 * b + 1];
+        else plan.mode = a.draft ? CM_BOTH : CM_P_LESS;
+        write();
+        if (plan.mode == CM_DONE) return plan;
+        if (accepted) {                                      // the sums of the rows behind it
+            const T *pr = chain_row<T>(a, b, plan.acc), *qr = plan.mode == CM_BOTH ? chain_row<T>(a, b, a.n + 1 + plan.acc) : nullptr;
+            sums_here(pr, qr, false, 0.0, 0.0, tp, tq);
+            if (plan.mode == CM_P_LESS) take_out(pr, tokens[plan.acc]);
+            double none;
+            if (qr) sums_here(pr, qr, true, 1.0 / tp, 1.0 / tq, qx, none);
+        }
+    }
     if (plan.mode == CM_SLOW) {
         // the walk on from the draft that was too near, every decision from fp64 sums
         const int cnt = chain_count(a, b);
@@ -485,21 +534,36 @@ __global__ void __launch_bounds__(kPickThreads) k_chain_pick(ChainArgs a, ChainS
                 sums_here(pr, qr, true, 1.0 / tp, 1.0 / tq, tq, none);
             } else if (!a.draft) {
                 plan.mode = CM_P_LESS;
-                if (in && tid == 0) {                        // the refused token out of its piece
-                    double y = 0.0;
-                    const int k = x / sc.piece;
-                    for (int j = k * sc.piece; j < min(a.V, (k + 1) * sc.piece); ++j)
-                        if (j != x) y += weigh(to_float(pr[j]), plan.mp);
-                    sp[k] = y;
-                }
-                __syncthreads();
+                take_out(pr, x);
             }
             break;
         }
-        int *out = a.out_tokens + (size_t)b * (a.n + 1);
-        for (int i = tid; i <= a.n; i += kPickThreads) out[i] = i < plan.acc ? tokens[i] : -1;
-        if (tid == 0) a.accepted[b] = plan.acc;
-        __syncthreads();
+        write();
+        if (plan.mode == CM_DONE) return plan;
+    }
+    return plan;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPickThreads, 1) k_chain_pick(const __grid_constant__ ChainArgs a, const __grid_constant__ ChainScratch sc) {
+    __shared__ double s_tab[64], s_sum[2][kPickThreads / 32];
+    __shared__ int s_pick, s_last;
+    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int pieces = sc.pieces;
+    const Weigh weigh = chain_weigh(a, b, s_tab);
+    const double *u = a.u + (size_t)b * (a.n + 1);
+    const int *tokens = a.tokens + (size_t)b * a.n;
+    if (tid == 0) {
+        s_pick = INT_MAX;
+        s_last = -1;
+    }
+    __syncthreads();
+    griddep_wait();
+    ChainPlan plan = sc.plan[2 * b];
+    if (plan.mode == CM_DONE) return;
+    double *sp = sc.sp + (size_t)b * pieces, *sq = sc.sq + (size_t)b * pieces, *left = sc.left + (size_t)b * pieces;
+    if (plan.mode >= CM_NEAR) {
+        plan = settle_near<T>(a, sc, b, s_tab, s_sum);
         if (plan.mode == CM_DONE) return;
     }
     const T *pr = chain_row<T>(a, b, plan.acc), *qr = plan.mode == CM_BOTH ? chain_row<T>(a, b, a.n + 1 + plan.acc) : nullptr;
@@ -598,7 +662,7 @@ ChainScratch chain_scratch(const ChainArgs &a, void *base) {
     sc.pieces = (a.V + sc.piece - 1) / sc.piece;
     const size_t pieces = (size_t)a.B * sc.pieces * sizeof(double);
     sc.st = reinterpret_cast<ChainStat *>(take((size_t)a.B * (2 * a.n + 1) * sc.chunks * sizeof(ChainStat)));
-    sc.plan = reinterpret_cast<ChainPlan *>(take((size_t)a.B * sizeof(ChainPlan)));
+    sc.plan = reinterpret_cast<ChainPlan *>(take((size_t)a.B * 2 * sizeof(ChainPlan)));
     sc.sp = reinterpret_cast<double *>(take(pieces));
     sc.sq = reinterpret_cast<double *>(take(pieces));
     sc.left = reinterpret_cast<double *>(take(pieces));

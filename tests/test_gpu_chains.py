@@ -139,6 +139,33 @@ def test_numbers_next_to_the_border_are_decided_in_64_bits(drafter):
     assert set(got[1]) >= {0, 1, 2} if not drafter else True
 
 
+@pytest.mark.parametrize("drafter", [True, False])
+@pytest.mark.parametrize("V", [40, 5000, 50001])
+def test_one_number_next_to_the_border(drafter, V):
+    """As above for one draft of a chain: accepted ones before it, and behind it all kinds (accepted, refused, a row without
+    weight), which follow only if it is accepted."""
+    B, n = 24, 3
+    target, draft, drafts, u = case(B, n, V, torch.float32, seed=19 + V, spread=1.0, near=0.3)
+    u[:, :n] = torch.rand(B, n, generator=torch.Generator().manual_seed(V), dtype=torch.float64)
+    if not drafter:
+        draft = None
+        drafts = target[:, :n].argmax(-1).int()
+    near, border = [b % n for b in range(B)], []
+    for b in range(B):
+        i, x = near[b], int(drafts[b, near[b]])
+        dist = lambda row: torch.softmax(row.double() / 0.7, 0)  # noqa: E731
+        p, q = float(dist(target[b, i])[x]), float(dist(draft[b, i])[x]) if drafter else 1.0
+        border.append(p < 0.99 * q)                      # else any number accepts it
+        u[b, :i] = 1e-9                                  # accepted, whatever p and q
+        u[b, i] = min(p / q, 0.999999) * (1 + (1e-6 if b // n % 2 else -1e-6))
+        if b >= 18:
+            target[b, i + 1] = -math.inf                 # behind it: nothing to accept or draw
+    temperature = torch.full((B,), 0.7)
+    got = run(target, draft, drafts, u, None, temperature)
+    assert got == oracle.chains(target, draft, drafts, u, None, temperature)
+    assert sum(border) >= 6 and all((got[1][b] > near[b]) == (b // n % 2 == 0) for b in range(B) if border[b])
+
+
 def test_strided_rows_and_rows_behind_the_counts_are_not_read():
     target, draft, drafts, u = case(3, 3, 999, torch.float32, seed=13)
     counts = torch.tensor([1, 3, 0], dtype=torch.int32)
