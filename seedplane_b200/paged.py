@@ -64,6 +64,7 @@ class PagedKV:
         if not k.is_cuda or (k.numel() > 0 and k.stride(4) != 1):
             raise ValueError("pages must be CUDA tensors with unit stride in the last dimension")
         self.k, self.v, self.device = k, v, k.device
+        self._index = k.get_device()
         self.layers, self.n_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         self._word = torch.zeros(1, dtype=torch.int32, device=k.device)
         self._layer = []
@@ -96,7 +97,7 @@ class PageBatch:
                  tokens: Optional[int] = None, max_q: int = 1, prefix_table: Optional[torch.Tensor] = None,
                  prefix_len: int = 0):
         dev = lens.device
-        self.device = dev
+        self.device, self._index = dev, lens.get_device()
         self.lens = _int32(lens, "lens", dev, 1)
         self.tables = _int32(tables, "tables", dev, 2)
         b = lens.numel()
@@ -124,7 +125,7 @@ class PageBatch:
     def _check(self, pages: PagedKV, layer: int):
         if not 0 <= layer < pages.layers:
             raise ValueError(f"layer {layer} of {pages.layers}")
-        if pages.device != self.device:
+        if pages._index != self._index:
             raise ValueError(f"pages on {pages.device}, batch on {self.device}")
         if self.prefix_len > self.prefix_pages * pages.page_size:
             raise ValueError(f"a prefix of {self.prefix_len} keys in {self.prefix_pages} pages of {pages.page_size}")
@@ -132,7 +133,7 @@ class PageBatch:
 
 def _rows(t: torch.Tensor, name: str, batch: PageBatch, cols: int) -> int:
     """The row stride of a [rows, ...] matrix of `cols` values a row (heads and dims contiguous)."""
-    if t.device != batch.device or t.dtype not in _TYPES:
+    if t.get_device() != batch._index or t.dtype not in _TYPES:
         raise ValueError(f"{name}: fp32, fp16 or bf16 on {batch.device} expected")
     if t.dim() < 2 or t.size(0) < batch.tokens or t.numel() != t.size(0) * cols:
         raise ValueError(f"{name}: [{batch.tokens}, {cols}] expected, not {tuple(t.shape)}")
@@ -160,18 +161,18 @@ def append(pages: PagedKV, layer: int, batch: PageBatch, qkv: torch.Tensor, head
     qs = _rows(q_out, "q_out", batch, heads * hd)
     if q_out.dtype != qkv.dtype:
         raise ValueError("q_out must have qkv's type")
-    if rope.dtype != torch.float32 or rope.device != batch.device or rope.dim() != 3 or rope.shape[2] != 2 or \
+    if rope.dtype != torch.float32 or rope.get_device() != batch._index or rope.dim() != 3 or rope.size(2) != 2 or \
             not rope.is_contiguous():
         raise ValueError("rope: contiguous fp32 [positions, rot_dim / 2, 2] expected")
-    if bias is not None and (bias.dtype != torch.float32 or bias.device != batch.device or bias.numel() != cols or
+    if bias is not None and (bias.dtype != torch.float32 or bias.get_device() != batch._index or bias.numel() != cols or
                              not bias.is_contiguous()):
         raise ValueError(f"bias: contiguous fp32 [{cols}] expected")
     if positions is not None and _int32(positions, "positions", batch.device, 1).numel() < batch.tokens:
         raise ValueError(f"positions: {batch.tokens} entries expected")
     N.check(N.load().sp_pages_append(
-        batch.device.index, pages._ref[layer], batch._ref, heads, qkv.data_ptr(), _TYPES[qkv.dtype], xs,
-        None if bias is None else bias.data_ptr(), rope.data_ptr(), rope.shape[0], 2 * rope.shape[1], int(interleaved),
-        None if positions is None else positions.data_ptr(), q_out.data_ptr(), qs, _raw_stream(batch.device.index)))
+        batch._index, pages._ref[layer], batch._ref, heads, qkv.data_ptr(), _TYPES[qkv.dtype], xs,
+        None if bias is None else bias.data_ptr(), rope.data_ptr(), rope.size(0), 2 * rope.size(1), int(interleaved),
+        None if positions is None else positions.data_ptr(), q_out.data_ptr(), qs, _raw_stream(batch._index)))
     return q_out
 
 
@@ -191,7 +192,7 @@ def attention(pages: PagedKV, layer: int, batch: PageBatch, q: torch.Tensor, *, 
     os_ = _rows(out, "out", batch, heads * pages.head_dim)
     if out.dtype != q.dtype:
         raise ValueError("out must have q's type")
-    if lse is not None and (lse.dtype != torch.float32 or lse.device != batch.device or lse.shape != (q.size(0), heads) or
+    if lse is not None and (lse.dtype != torch.float32 or lse.get_device() != batch._index or lse.shape != (q.size(0), heads) or
                             not lse.is_contiguous()):
         raise ValueError(f"lse: contiguous fp32 [{q.shape[0]}, {heads}] expected")
     lib, c, dt = N.load(), pages._ref[layer], _TYPES[q.dtype]
@@ -204,7 +205,7 @@ def attention(pages: PagedKV, layer: int, batch: PageBatch, q: torch.Tensor, *, 
         batch._ws[key] = need
     ws = torch.empty(need, dtype=torch.uint8, device=batch.device) if need else None
     N.check(lib.sp_pages_attention(
-        batch.device.index, c, batch._ref, heads, q.data_ptr(), dt, qs, scale if scale is not None else pages.head_dim ** -0.5,
+        batch._index, c, batch._ref, heads, q.data_ptr(), dt, qs, scale if scale is not None else pages.head_dim ** -0.5,
         out.data_ptr(), os_, None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), need,
-        _raw_stream(batch.device.index)))
+        _raw_stream(batch._index)))
     return out

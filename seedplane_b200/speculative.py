@@ -273,7 +273,7 @@ def accept_chains(target_logits, draft_logits, drafts, u, *, counts=None, temper
     drawn one, then -1; accepted int32 [B]); `out`: that pair's tensors to write into."""
     import torch
     from .paged import N, _TYPES, _raw_stream
-    dev = target_logits.device
+    dev = target_logits.get_device()                      # cheaper than a torch.device, as are the other checks' forms
     dtype = _TYPES.get(target_logits.dtype)
     if target_logits.dim() != 3 or not target_logits.is_cuda or dtype is None or target_logits.stride(2) != 1:
         raise ValueError("target_logits: fp32, fp16 or bf16 [B, n + 1, V] on a CUDA device, rows contiguous, expected")
@@ -281,21 +281,21 @@ def accept_chains(target_logits, draft_logits, drafts, u, *, counts=None, temper
     n = n1 - 1
     draft, dbs, dld = None, 0, 0
     if draft_logits is not None:
-        if draft_logits.shape != (B, n, V) or draft_logits.dtype != target_logits.dtype or draft_logits.device != dev or \
+        if draft_logits.shape != (B, n, V) or draft_logits.dtype != target_logits.dtype or draft_logits.get_device() != dev or \
                 (n > 0 and draft_logits.stride(2) != 1):
             raise ValueError(f"draft_logits: [{B}, {n}, {V}] like target_logits expected")
         draft, dbs, dld = draft_logits.data_ptr(), draft_logits.stride(0), draft_logits.stride(1) if n > 1 else V
 
     def need(t, name, want, shape):
-        if t.dtype != want or t.device != dev or t.shape != shape or not t.is_contiguous():
-            raise ValueError(f"{name}: contiguous {want} {list(shape)} on {dev} expected")
+        if t.dtype is not want or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"{name}: contiguous {want} {list(shape)} on cuda:{dev} expected")
         return t.data_ptr()
 
     drafts_at = need(drafts, "drafts", torch.int32, (B, n))
     u_at = need(u, "u", torch.float64, (B, n1))
     counts_at = None if counts is None else need(counts, "counts", torch.int32, (B,))
     if temperature is not None and not isinstance(temperature, torch.Tensor):
-        temperature = torch.full((B,), float(temperature), dtype=torch.float32, device=dev)
+        temperature = torch.full((B,), float(temperature), dtype=torch.float32, device=target_logits.device)
     temperature_at = None if temperature is None else need(temperature, "temperature", torch.float32, (B,))
     lib = N.load()
     size = lib.sp_accept_chains_workspace(B, n, V)
@@ -309,8 +309,8 @@ def accept_chains(target_logits, draft_logits, drafts, u, *, counts=None, temper
         tokens_at = need(out[0], "out tokens", torch.int32, (B, n1))
         accepted_at = need(out[1], "out accepted", torch.int32, (B,))
     N.check(lib.sp_accept_chains(
-        dev.index, B, n, V, target_logits.data_ptr(), target_logits.stride(0), target_logits.stride(1) if n else V, draft, dbs, dld, dtype,
-        drafts_at, counts_at, u_at, temperature_at, tokens_at, accepted_at, ws.data_ptr(), size, _raw_stream(dev.index)))
+        dev, B, n, V, target_logits.data_ptr(), target_logits.stride(0), target_logits.stride(1) if n else V, draft, dbs, dld, dtype,
+        drafts_at, counts_at, u_at, temperature_at, tokens_at, accepted_at, ws.data_ptr(), size, _raw_stream(dev)))
     return out
 
 
