@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(kStatThreads) k_chain_stats(ChainArgs a, Chain
 
 // ---- exponentials in 64 bits -------------------------------------------------------------------
 // Table-driven (Tang 1989): z / (ln 2 / 64) = n + f, |f| <= 1/2, by adding 1.5 2^52; e^z = 2^(n >> 6) 2^((n & 63) / 64)
-// e^(f ln 2 / 64), the last by its Taylor polynomial of degree 4 (relative error below 4e-14). Eleven fp64
+// e^(f ln 2 / 64), the last by its Taylor polynomial of degree 4 (relative error below 4e-14). Twelve fp64
 // operations.
 __constant__ double c_exp_tab[64] = {         // 2^(i / 64)
     0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0, 0x1.0b5586cf9890fp+0,
@@ -181,7 +181,10 @@ struct Weigh {                               // exp((l - max) / T) of a row's lo
     // without a branch, so that several are under way in a thread
     SP_DEVINL double operator()(float l, float m) const {
         const bool some = (l - m) * k2 > -1000.f;            // no for NaN, -inf and an infinite maximum
-        const double y = fma((double)l, k, -((double)m * k));   // m k is rounded once for the row
+        // (l - m) k, with what the rounding of m k left off taken back (by the row): 0 at the maximum whatever T and the
+        // logits' size, where at T = 1e-15, or logits of 1e20, that rest alone is as large as the exponent may be. The
+        // difference first takes one operation less and 8 more registers: 54.5 against 52.4 us for 48 requests
+        const double mk = (double)m * k, y = fma((double)l, k, -mk) - fma((double)m, k, -mk);
         const double t = y + 0x1.8p52;
         const int n = __double2loint(t);
         const double f = y - (t - 0x1.8p52);
