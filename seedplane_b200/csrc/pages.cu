@@ -248,6 +248,10 @@ cudaError_t append_typed(const PagesAppend &p, cudaStream_t s) {
 // the prefix beside it).
 constexpr int kRowsWarps = 4, kRowsStages = 2;
 constexpr int kRowsTileBytes = 4096;                         // K (or V) rows of one warp's tile
+// m lies this far (in base 2) below the running maximum: probabilities are at most 2^14, and what fp16's subnormals round
+// off is 2^-39 of the maximum's and not 2^-25 (bf16 has fp32's range)
+template <typename TC>
+constexpr float kRowsBias = std::is_same<TC, __half>::value ? 14.0f : 0.0f;
 constexpr int kRowsSmem = kRowsWarps * kRowsStages * 2 * kRowsTileBytes;
 
 template <int HD>
@@ -494,7 +498,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 3) k_pages_rows(PagesAttentio
         for (int i = 0; i < NR; ++i) {
             mt[i] = fmaxf(mt[i], __shfl_xor_sync(0xffffffffu, mt[i], 1));
             mt[i] = fmaxf(mt[i], __shfl_xor_sync(0xffffffffu, mt[i], 2));
-            const float mn = fmaxf(m[i], mt[i] * sc);
+            const float mn = fmaxf(m[i], fmaf(mt[i], sc, -kRowsBias<TC>));
             ms[i] = mn == -INFINITY ? 0.f : mn;              // a row that has seen no key yet
             corr[i] = exp2_approx(m[i] - ms[i]);
             m[i] = mn;

@@ -4,9 +4,9 @@
 // A CTA takes up to 256 (token, head) rows of one kv head's group and walks a key sequence (a range of the
 // prefix, or the prefix and then one request's own keys) in tiles of 128 keys:
 //   S_q = Q_q K^T    tcgen05.mma M 128, N 128 into TMEM (two row tiles q, 128 columns each)
-//   P_q = 2^(S c - m), m the row's running maximum, kept while it grows by less than 2^8, so that the sums
-//         and O seldom need rescaling (P <= 256 then, within either 16-bit type's range); written over
-//         S_q in TMEM in the cache's type
+//   P_q = 2^(S c - m), m the row's running maximum (less a bias), kept while it grows by less than 2^8 (2^4 with fp32
+//         queries), so that the sums and O seldom need rescaling (P <= 2^15 then, within either 16-bit type's range);
+//         written over S_q in TMEM in the cache's type
 //   O_q += P_q V     tcgen05.mma with A = P_q in TMEM, B = V as it lies in its pages (MN-major)
 // Packed prompts (12 requests, 3,679 rows x 28 heads over 3,001 + 560 keys) take 195 us, 917 TFLOP/s, at the 1,000 W
 // cap (1.8 GHz); the MMAs alone take 127 us, with the tiles' loads 151, the softmax with the loads 176. A row tile's
@@ -45,7 +45,15 @@ constexpr int kTcProducer = 16, kTcMma = 17; // warps
 constexpr int kTcStages = 4;
 constexpr uint32_t kTcSpin = 1u << 22;
 constexpr int kTcFlush = 2;                  // fp32 queries: O is added up in fp32 outside the MMAs every so many tiles
-constexpr float kTcGrow = 8.0f;              // log2 of the growth a running maximum may lag behind
+// A row's probabilities are 2^(its scores - m), m kTcBias below a running maximum that may lag behind by kTcGrow (all in
+// base 2). In fp16 they end at 2^15, and its subnormals' rounding, 2^-25, lies kTcBias further below the maximum: without
+// it many small weights behind a large one (a key that takes most of the weight and has a value near 0) lose their bits.
+// A shorter lag means a longer bias and more rescaling: none for fp16 queries (prompts 196 us, with a lag of 4 207), but
+// fp32 ones carry a lo half too (prompts 465 us with a lag of 8, 481 with 4, 490 with 2). bf16 has fp32's range.
+template <typename TQ, typename TC>
+constexpr float kTcGrow = std::is_same<TC, __half>::value && sizeof(TQ) == 4 ? 4.0f : 8.0f;
+template <typename TQ, typename TC>
+constexpr float kTcBias = std::is_same<TC, __half>::value ? 15.0f - kTcGrow<TQ, TC> : 0.0f;
 
 template <int HD>
 struct TcSmem {
@@ -501,8 +509,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         mx[1] = max3(mx[1], __uint_as_float(s[j + 2]), __uint_as_float(s[j + 3]));
                     }
                 }
-                const float mine = fmaxf(mx[0], mx[1]), mt = fmaxf(mine, swap(mine)) * c;
-                const bool grow = mt > m + kTcGrow || (!any && mt > m);
+                const float mine = fmaxf(mx[0], mx[1]), mt = fmaf(fmaxf(mine, swap(mine)), c, -kTcBias<TQ, TC>);
+                const bool grow = mt > m + kTcGrow<TQ, TC> || (!any && mt > m);
                 const bool flush = kSplit && !alt && i > 0 && i % kTcFlush == 0;
                 if (any && (flush || __any_sync(0xffffffffu, grow))) {
                     // s_full of this tile came after the products of the tile before: O is at rest
