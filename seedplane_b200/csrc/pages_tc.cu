@@ -422,8 +422,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     } else {
         const int grp = warp >> 3, half = (warp >> 2) & 1;
         const TQ *qbase = reinterpret_cast<const TQ *>(p.q);
-        // Q rows into swizzled tiles (rows behind the last: zero), a batch of loads under way at once
-        const int fill = (alt || nq == 1 ? 1 : 2) * kTcRows * CH;
+        // Q rows into swizzled tiles (rows behind the last: zero), a batch of loads under way at once. Without a key
+        // nothing reads them, and no product stands between these stores and the rows that leave through the same memory
+        const int fill = n == 0 ? 0 : (alt || nq == 1 ? 1 : 2) * kTcRows * CH;
         constexpr int QB = kSplit ? 4 : 8;
         for (int i0 = tid; i0 < fill; i0 += kTcSoftmax * QB) {
             uint4 v[QB], v2[kSplit ? QB : 1];
