@@ -48,9 +48,9 @@ SP_DEVINL float exp2_approx(float x) {                       // 2^x, relative er
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// log-sum-exp of a row from its base-2 maximum and sum
+// log-sum-exp of a row from its base-2 maximum and sum; no sum: no key. A row of NaN scores has a sum (NaN), but no maximum
 SP_DEVINL float row_lse(float m, float l) {
-    return m == -INFINITY ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+    return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
 // ---- the ragged batch --------------------------------------------------------------------------
