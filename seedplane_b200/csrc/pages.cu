@@ -248,8 +248,8 @@ cudaError_t append_typed(const PagesAppend &p, cudaStream_t s) {
 // the prefix beside it).
 constexpr int kRowsWarps = 4, kRowsStages = 2;
 constexpr int kRowsTileBytes = 4096;                         // K (or V) rows of one warp's tile
-// m lies this far (in base 2) below the running maximum: probabilities are at most 2^14, and what fp16's subnormals round
-// off is 2^-39 of the maximum's and not 2^-25 (bf16 has fp32's range)
+// Probabilities are held times 2^kRowsBias: at most 2^14, and what fp16's subnormals round off is 2^-39 of the maximum's
+// and not 2^-25 (bf16 has fp32's range)
 template <typename TC>
 constexpr float kRowsBias = std::is_same<TC, __half>::value ? 14.0f : 0.0f;
 constexpr int kRowsSmem = kRowsWarps * kRowsStages * 2 * kRowsTileBytes;
@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 3) k_pages_rows(PagesAttentio
     }
     // own keys each row sees: below this
     const int sa = own0 + ra / G + 1, sb = own0 + rb / G + 1;
-    const float sc = p.scale * 1.4426950408889634f;
+    const float sc = row_scale(p);
     float o[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
@@ -498,9 +498,9 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 3) k_pages_rows(PagesAttentio
         for (int i = 0; i < NR; ++i) {
             mt[i] = fmaxf(mt[i], __shfl_xor_sync(0xffffffffu, mt[i], 1));
             mt[i] = fmaxf(mt[i], __shfl_xor_sync(0xffffffffu, mt[i], 2));
-            const float mn = fmaxf(m[i], fmaf(mt[i], sc, -kRowsBias<TC>));
+            const float mn = fmaxf(m[i], mt[i]);
             ms[i] = mn == -INFINITY ? 0.f : mn;              // a row that has seen no key yet
-            corr[i] = exp2_approx(m[i] - ms[i]);
+            corr[i] = max_factor(m[i], mn, sc);
             m[i] = mn;
             l[i] *= corr[i];
         }
@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 3) k_pages_rows(PagesAttentio
         for (int nt = 0; nt < ST; ++nt) {
             float e[4];
 #pragma unroll
-            for (int i = 0; i < 2 * NR; ++i) e[i] = exp2_approx(fmaf(s[nt][i], sc, -ms[i >> 1]));
+            for (int i = 0; i < 2 * NR; ++i) e[i] = exp2_approx(fmaf(s[nt][i] - ms[i >> 1], sc, kRowsBias<TC>));
             l[0] += e[0] + e[1];
             uint32_t hi = pack2<TC>(e[0], e[1]), lo;
             if constexpr (kSplit) {
@@ -586,7 +586,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 3) k_pages_rows(PagesAttentio
     for (int d = 0; d < DPT; ++d) acc[d] = 0.f;
 #pragma unroll
     for (int w = 0; w < kRowsWarps; ++w) {
-        const float f = exp2_approx(sm[(w * RT + r) * 2] - Ms);
+        const float f = exp2_approx(fmaf(sm[(w * RT + r) * 2] - Ms, sc, -kRowsBias<TC>));
         L = fmaf(sm[(w * RT + r) * 2 + 1], f, L);
 #pragma unroll
         for (int d = 0; d < DPT; ++d) acc[d] = fmaf(so[(w * RT + r) * OS + d0 + d], f, acc[d]);
@@ -597,7 +597,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 3) k_pages_rows(PagesAttentio
         TQ *dst = reinterpret_cast<TQ *>(p.out) + rt * p.out_stride + hh * HD + d0;
 #pragma unroll
         for (int d = 0; d < DPT; ++d) dst[d] = from_float<TQ>(L == L ? acc[d] * inv : L);
-        if (p.lse && d0 == 0) p.lse[rt * p.nh + hh] = row_lse(M, L);
+        if (p.lse && d0 == 0) p.lse[rt * p.nh + hh] = row_lse(M, L, sc);
     } else {
         const long long at = ((long long)slot * ba.T + rt) * p.nh + hh;
         float *dst = pl.acc + at * HD + d0;
@@ -636,10 +636,10 @@ __global__ void __launch_bounds__(32 * kMergeWarps) k_pages_merge(PagesAttention
         M = fmaxf(M, ml[i].x);
     }
     M = warp_max(M);
-    const float Ms = M == -INFINITY ? 0.f : M;
+    const float Ms = M == -INFINITY ? 0.f : M, sc = row_scale(p);
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
-        const float f = exp2_approx(ml[i].x - Ms);
+        const float f = exp2_approx((ml[i].x - Ms) * sc);
         L = fmaf(ml[i].y, f, L);
         if (warp == 0) s_w[32 * i + lane] = f;
     }
@@ -686,7 +686,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) k_pages_merge(PagesAttention
         for (int w = 0; w < kMergeWarps; ++w) v += s_acc[w][d];
         reinterpret_cast<TQ *>(p.out)[(long long)t * p.out_stride + h * HD + d] = from_float<TQ>(L == L ? v * inv : L);
     }
-    if (p.lse && threadIdx.x == 0) p.lse[at] = row_lse(M, L);
+    if (p.lse && threadIdx.x == 0) p.lse[at] = row_lse(M, L, sc);
 }
 
 // The same with a warp per (token, head), for at most 32 ranges: no shared memory, no barrier. Where a CTA per (token,
@@ -703,7 +703,8 @@ __global__ void __launch_bounds__(32 * kMergeWarps) k_pages_merge_few(PagesAtten
     griddep_wait();
     if (none) return;
     const float2 ml = lane < pl.slots ? *reinterpret_cast<const float2 *>(pl.ml + (lane * step + at) * 2) : make_float2(-INFINITY, 0.f);
-    const float M = warp_max(ml.x), w = exp2_approx(ml.x - (M == -INFINITY ? 0.f : M)), L = warp_sum(ml.y * w);
+    const float M = warp_max(ml.x), sc = row_scale(p), w = exp2_approx((ml.x - (M == -INFINITY ? 0.f : M)) * sc);
+    const float L = warp_sum(ml.y * w);
     float acc[DL];
 #pragma unroll
     for (int d = 0; d < DL; ++d) acc[d] = 0.f;
@@ -745,7 +746,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) k_pages_merge_few(PagesAtten
         if constexpr (DL == 4) *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2<TQ>(acc[0], acc[1]), pack2<TQ>(acc[2], acc[3]));
         else *reinterpret_cast<uint32_t *>(dst) = pack2<TQ>(acc[0], acc[1]);
     }
-    if (p.lse && lane == 0) p.lse[at] = row_lse(M, L);
+    if (p.lse && lane == 0) p.lse[at] = row_lse(M, L, sc);
 }
 
 // Which kernel takes what. k_pages_tc pads a row tile to 128 rows and needs an SM to itself; k_pages_rows reads K and

@@ -48,10 +48,16 @@ SP_DEVINL float exp2_approx(float x) {                       // 2^x, relative er
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// log-sum-exp of a row from its base-2 maximum and sum; no sum: no key. A row of NaN scores has a sum (NaN), but no maximum
-SP_DEVINL float row_lse(float m, float l) {
-    return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+// A row's (or a key range's) statistics: m, its largest q k before the scale, and l, the sum of 2^((q k - m) c), c = scale
+// log2(e). The difference is taken before the product: it is 0 at the maximum, however large the scores are (a rounded
+// m c leaves up to 2^-24 of itself there).
+// The log-sum-exp; no sum: no key. A row of NaN scores has a sum (NaN), but no maximum
+SP_DEVINL float row_lse(float m, float l, float c) {
+    return l == 0.f ? -INFINITY : fmaf(m, c, log2f(l)) * 0.6931471805599453f;
 }
+SP_DEVINL float row_scale(const PagesAttention &p) { return p.scale * 1.4426950408889634f; }
+// 2^((a - b) c) of two maxima a <= b, -inf where there was no key: 1 for none at all
+SP_DEVINL float max_factor(float a, float b, float c) { return b == -INFINITY ? 1.f : exp2_approx((a - b) * c); }
 
 // ---- the ragged batch --------------------------------------------------------------------------
 SP_DEVINL void set_status(int *status) {

@@ -4,7 +4,7 @@
 // A CTA takes up to 256 (token, head) rows of one kv head's group and walks a key sequence (a range of the
 // prefix, or the prefix and then one request's own keys) in tiles of 128 keys:
 //   S_q = Q_q K^T    tcgen05.mma M 128, N 128 into TMEM (two row tiles q, 128 columns each)
-//   P_q = 2^(S c - m), m the row's running maximum (less a bias), kept while it grows by less than 2^8 (2^4 with fp32
+//   P_q = 2^((S - m) c + bias), m the row's running maximum, kept while it grows by less than 2^8 (2^4 with fp32
 //         queries), so that the sums and O seldom need rescaling (P <= 2^15 then, within either 16-bit type's range);
 //         written over S_q in TMEM in the cache's type
 //   O_q += P_q V     tcgen05.mma with A = P_q in TMEM, B = V as it lies in its pages (MN-major)
@@ -45,8 +45,8 @@ constexpr int kTcProducer = 16, kTcMma = 17; // warps
 constexpr int kTcStages = 4;
 constexpr uint32_t kTcSpin = 1u << 22;
 constexpr int kTcFlush = 2;                  // fp32 queries: O is added up in fp32 outside the MMAs every so many tiles
-// A row's probabilities are 2^(its scores - m), m kTcBias below a running maximum that may lag behind by kTcGrow (all in
-// base 2). In fp16 they end at 2^15, and its subnormals' rounding, 2^-25, lies kTcBias further below the maximum: without
+// A row's probabilities are held times 2^kTcBias, and its running maximum may lag behind by kTcGrow (in base 2). In fp16
+// they end at 2^15, and its subnormals' rounding, 2^-25, lies kTcBias further below the maximum: without
 // it many small weights behind a large one (a key that takes most of the weight and has a value near 0) lose their bits.
 // A shorter lag means a longer bias and more rescaling: none for fp16 queries (prompts 196 us, with a lag of 4 207), but
 // fp32 ones carry a lo half too (prompts 465 us with a lag of 8, 481 with 4, 490 with 2). bf16 has fp32's range.
@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int seen = live ? own0 + row / G + 1 : 0;  // own keys this row sees: below this
             const uint32_t lanes = (uint32_t)(warp & 3) * 32u << 16;
             const uint32_t ts = tmem + lanes + 128u * grp, to = tmem + lanes + 256u + 128u * grp;
-            const float c = p.scale * 1.4426950408889634f;
+            const float c = row_scale(p);
             float m = -INFINITY, l = 0.f;
             uint32_t ph = 0u;
             bool ok = true, any = false, flushed = false;
@@ -510,12 +510,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         mx[1] = max3(mx[1], __uint_as_float(s[j + 2]), __uint_as_float(s[j + 3]));
                     }
                 }
-                const float mine = fmaxf(mx[0], mx[1]), mt = fmaf(fmaxf(mine, swap(mine)), c, -kTcBias<TQ, TC>);
-                const bool grow = mt > m + kTcGrow<TQ, TC> || (!any && mt > m);
+                const float mine = fmaxf(mx[0], mx[1]), mt = fmaxf(mine, swap(mine));
+                const bool grow = (mt - m) * c > kTcGrow<TQ, TC> || (!any && mt > m);
                 const bool flush = kSplit && !alt && i > 0 && i % kTcFlush == 0;
                 if (any && (flush || __any_sync(0xffffffffu, grow))) {
                     // s_full of this tile came after the products of the tile before: O is at rest
-                    const float f = grow ? exp2_approx(m - mt) : 1.f;
+                    const float f = grow ? max_factor(m, mt, c) : 1.f;
                     l *= f;
 #pragma unroll 1
                     for (int k = 0; k < HD / 32; ++k) {
@@ -541,7 +541,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (grow) m = mt;
                 any = true;
                 const float ms = m == -INFINITY ? 0.f : m;
-                const uint64_t c2 = f2(c, c), m2 = f2(-ms, -ms);
+                // the difference costs an instruction for two columns (packed prompts 196.5 -> 199 us); a second loop
+                // without it, for scores small enough, took 211
+                const uint64_t c2 = f2(c, c), m2 = f2(-ms, -ms), k2 = f2(kTcBias<TQ, TC>, kTcBias<TQ, TC>);
                 uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
@@ -549,7 +551,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     scores(k, s);
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
-                        const uint64_t x = fma2((uint64_t)s[2 * j] | ((uint64_t)s[2 * j + 1] << 32), c2, m2);
+                        const uint64_t x = fma2(add2((uint64_t)s[2 * j] | ((uint64_t)s[2 * j + 1] << 32), m2), c2, k2);
                         const float e0 = exp2_approx(f2_lo(x)), e1 = exp2_approx(f2_hi(x));
                         sum[j & 1] = add2(sum[j & 1], f2(e0, e1));
                         hi[j] = pack2<TC>(e0, e1);
@@ -577,11 +579,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             for (int q = 0; q < nq; ++q)
                 if (ok && (alt ? q < n : n > 0)) ok = w.wait_warp(&bar.o_full[q], 0);
             tc_fence_after();
-            l += swap(l);
+            constexpr float kUnbias = 1.0f / (1 << (int)kTcBias<TQ, TC>);
+            l = (l + swap(l)) * kUnbias;
             const long long rt = q0 + row / G, hh = g * G + row % G;
             const long long at = ((long long)(slot + (alt ? grp : 0)) * ba.T + rt) * p.nh + hh;
             const bool direct = pl.slots == 1;
-            const float inv = l > 0.f ? 1.f / l : 0.f;
+            const float out = (!direct ? 1.f : l > 0.f ? 1.f / l : 0.f) * kUnbias;
             constexpr int HALF = HD / 2, STRIDE = HALF * 4 + 16;
             const uint32_t stage = base + (uint32_t)warp * 32 * STRIDE;
 #pragma unroll
@@ -601,10 +604,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
                     for (int j = 0; j < 32; ++j) o[j] = 0u;
                 }
-                if (direct) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(l == l ? __uint_as_float(o[j]) * inv : l);
-                }
+                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(!direct || l == l ? __uint_as_float(o[j]) * out : l);
                 const uint32_t mine = stage + lane * STRIDE;
                 if (direct && !kSplit) {
 #pragma unroll
@@ -636,7 +637,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             if (live && half == 0) {
                 if (!direct) *reinterpret_cast<float2 *>(pl.ml + at * 2) = make_float2(m, l);
-                else if (p.lse) p.lse[rt * p.nh + hh] = row_lse(m, l);
+                else if (p.lse) p.lse[rt * p.nh + hh] = row_lse(m, l, c);
             }
             tc_fence_before();
         }
