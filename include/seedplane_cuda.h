@@ -288,7 +288,7 @@ int64_t sp_pages_attention_workspace(const sp_pages *pages, const sp_page_batch 
  * prefix's keys and the request's own keys up to the row's own; the prefix's pages are read once for
  * the whole batch. q, out: [row][heads * head_dim], q_stride / out_stride elements apart (multiples of
  * 8, 16-byte aligned). dtype of q and out: SP_F32 over SP_F16 pages (scores and values then carry the
- * queries and probabilities as two fp16 halves, ~22 bits), or the pages' own type (probabilities
+ * queries and probabilities as two fp16 halves: 2^-22 of each, and of a query 2^-39 of its row's largest), or the pages' own type (probabilities
  * rounded to it; sums, maxima and outputs fp32, rounded once). Over SP_F16 pages a probability is off by
  * 2^-36 (fp32 queries) or 2^-32 of the row's largest besides, fp16's least steps. A row that sees no key gives zeros. Slots that
  * hold no key may hold anything; the values of keys that another row of the request sees must be finite.

@@ -428,15 +428,29 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 3) k_pages_rows(PagesAttentio
     const bool la = gq < nrows, lb = kSplit ? la : gq + 8 < nrows;
     const TQ *qbase = reinterpret_cast<const TQ *>(p.q);
     const auto q_row = [&](int r) { return qbase + (long long)(q0 + r / G) * p.q_stride + (g * G + r % G) * HD; };
+    float up = 1.f;                                          // fp32 queries: what the row's were divided by
     {
         const TQ *pa = q_row(la ? ra : row0), *pb = q_row(lb ? rb : row0);
+        float down = 1.f;
+        float2 xs[kSplit ? 2 * KS : 1];                      // at dims 8 i + 2 tq
+        if constexpr (kSplit) {
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2 * KS; ++i) {
+                xs[i] = la ? *reinterpret_cast<const float2 *>(pa + 8 * i + 2 * tq) : make_float2(0.f, 0.f);
+                top = fmaxf(top, fmaxf(fabsf(xs[i].x), fabsf(xs[i].y)));
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            row_power(top, down, up);
+        }
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk) {
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
                 const int d = 16 * kk + 8 * hf + 2 * tq;
                 if constexpr (kSplit) {
-                    const float2 x = la ? *reinterpret_cast<const float2 *>(pa + d) : make_float2(0.f, 0.f);
+                    const float2 x = make_float2(xs[2 * kk + hf].x * down, xs[2 * kk + hf].y * down);
                     const __half ha = __float2half_rn(x.x), hb = __float2half_rn(x.y);
                     qa[kk][2 * hf] = pack2<__half>(x.x, x.y);
                     qa[kk][2 * hf + 1] = pack2<__half>(x.x - __half2float(ha), x.y - __half2float(hb));
@@ -449,7 +463,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 3) k_pages_rows(PagesAttentio
     }
     // own keys each row sees: below this
     const int sa = own0 + ra / G + 1, sb = own0 + rb / G + 1;
-    const float sc = row_scale(p);
+    const float sc = row_scale(p) * up;
     float o[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
@@ -567,7 +581,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 3) k_pages_rows(PagesAttentio
         }
     }
     if (tq == 0) {
-        sm[(warp * RT + gq) * 2] = m[0];
+        sm[(warp * RT + gq) * 2] = m[0] * up;
         sm[(warp * RT + gq) * 2 + 1] = l[0];
         if constexpr (!kSplit) {
             sm[(warp * RT + gq + 8) * 2] = m[1];
@@ -581,12 +595,12 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 3) k_pages_rows(PagesAttentio
     float M = -INFINITY, L = 0.f, acc[DPT];
 #pragma unroll
     for (int w = 0; w < kRowsWarps; ++w) M = fmaxf(M, sm[(w * RT + r) * 2]);
-    const float Ms = M == -INFINITY ? 0.f : M;
+    const float Ms = M == -INFINITY ? 0.f : M, c = kSplit ? row_scale(p) : sc;    // this row's own
 #pragma unroll
     for (int d = 0; d < DPT; ++d) acc[d] = 0.f;
 #pragma unroll
     for (int w = 0; w < kRowsWarps; ++w) {
-        const float f = exp2_approx(fmaf(sm[(w * RT + r) * 2] - Ms, sc, -kRowsBias<TC>));
+        const float f = exp2_approx(fmaf(sm[(w * RT + r) * 2] - Ms, c, -kRowsBias<TC>));
         L = fmaf(sm[(w * RT + r) * 2 + 1], f, L);
 #pragma unroll
         for (int d = 0; d < DPT; ++d) acc[d] = fmaf(so[(w * RT + r) * OS + d0 + d], f, acc[d]);
@@ -597,7 +611,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 3) k_pages_rows(PagesAttentio
         TQ *dst = reinterpret_cast<TQ *>(p.out) + rt * p.out_stride + hh * HD + d0;
 #pragma unroll
         for (int d = 0; d < DPT; ++d) dst[d] = from_float<TQ>(L == L ? acc[d] * inv : L);
-        if (p.lse && d0 == 0) p.lse[rt * p.nh + hh] = row_lse(M, L, sc);
+        if (p.lse && d0 == 0) p.lse[rt * p.nh + hh] = row_lse(M, L, c);
     } else {
         const long long at = ((long long)slot * ba.T + rt) * p.nh + hh;
         float *dst = pl.acc + at * HD + d0;

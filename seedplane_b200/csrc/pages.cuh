@@ -59,6 +59,14 @@ SP_DEVINL float row_scale(const PagesAttention &p) { return p.scale * 1.44269504
 // 2^((a - b) c) of two maxima a <= b, -inf where there was no key: 1 for none at all
 SP_DEVINL float max_factor(float a, float b, float c) { return b == -INFINITY ? 1.f : exp2_approx((a - b) * c); }
 
+// fp32 queries are split into fp16 halves after a power of two, exact to take back, that brings the row's largest |q| into
+// [2^14, 2^15): any finite query has halves then, and what the lo half rounds off is 2^-39 of the largest
+SP_DEVINL void row_power(float top, float &down, float &up) {
+    const int e = min(max((int)(__float_as_uint(top) >> 23), 28), 254) - 141;
+    down = __uint_as_float((uint32_t)(127 - e) << 23);
+    up = __uint_as_float((uint32_t)(127 + e) << 23);
+}
+
 // ---- the ragged batch --------------------------------------------------------------------------
 SP_DEVINL void set_status(int *status) {
     if (status) atomicCAS(status, 0, kErrPages);

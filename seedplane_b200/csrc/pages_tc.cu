@@ -166,6 +166,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
     __shared__ float s_swap[2][2][kTcRows];
+    __shared__ float s_up[kSplit ? kTcRows : 1];             // what a row's queries were divided by
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const PageBatchView &ba = p.ba;
     const int g = blockIdx.y, G = p.nh / p.pg.nkv;
@@ -447,9 +448,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if constexpr (kSplit) {
                     const uint32_t x[8] = {v[j].x, v[j].y, v[j].z, v[j].w, v2[j].x, v2[j].y, v2[j].z, v2[j].w};
                     uint32_t hw[4], lw[4];
+                    float top = 0.f, down, up;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(__uint_as_float(x[k])));
+#pragma unroll
+                    for (int k = CH / 2; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));    // a row's CH lanes
+                    row_power(top, down, up);
+                    if (c == 0) s_up[r] = up;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const float x0 = __uint_as_float(x[2 * k]), x1 = __uint_as_float(x[2 * k + 1]);
+                        const float x0 = __uint_as_float(x[2 * k]) * down, x1 = __uint_as_float(x[2 * k + 1]) * down;
                         float h0, h1;
                         hw[k] = pack2<TC>(x0, x1);
                         unpack2<TC>(hw[k], h0, h1);
@@ -463,6 +471,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
         }
         fence_proxy_async_smem();
+        if constexpr (kSplit) asm volatile("bar.sync 9, %0;" ::"n"(kTcSoftmax) : "memory");    // s_up
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar.q_full);
         if (grp < nq) {
@@ -471,7 +480,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int seen = live ? own0 + row / G + 1 : 0;  // own keys this row sees: below this
             const uint32_t lanes = (uint32_t)(warp & 3) * 32u << 16;
             const uint32_t ts = tmem + lanes + 128u * grp, to = tmem + lanes + 256u + 128u * grp;
-            const float c = row_scale(p);
+            const float up = kSplit && n > 0 ? s_up[r % (kSplit ? kTcRows : 1)] : 1.f, c = row_scale(p) * up;
             float m = -INFINITY, l = 0.f;
             uint32_t ph = 0u;
             bool ok = true, any = false, flushed = false;
@@ -636,7 +645,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (d) *reinterpret_cast<uint4 *>(d + c16) = v;
             }
             if (live && half == 0) {
-                if (!direct) *reinterpret_cast<float2 *>(pl.ml + at * 2) = make_float2(m, l);
+                if (!direct) *reinterpret_cast<float2 *>(pl.ml + at * 2) = make_float2(m * up, l);
                 else if (p.lse) p.lse[rt * p.nh + hh] = row_lse(m, l, c);
             }
             tc_fence_before();
