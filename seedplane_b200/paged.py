@@ -76,7 +76,7 @@ class PagedKV:
         self.layer_array = (N.SpPages * self.layers)(*self._layer)
         self._ref = [C.byref(c) for c in self._layer]
         # what a workspace's size depends on
-        self._key = (self.n_pages, self.page_size, self.kv_heads, k.dtype, k.stride()[1:])
+        self._key = (self.n_pages, self.page_size, self.kv_heads, self.head_dim, k.dtype, k.stride()[1:])
 
     def status(self):
         """Raise if a kernel met a bad page number, length or position since the last check (waits
