@@ -26,11 +26,15 @@ def token_sha256(tokens: List[int]) -> str:
 
 
 def native_generate(engine, payload: dict) -> dict:
-    """A `generate` request on a `NativeEngine` (text or token ids), the reference agent's result."""
+    """A `generate` request on a `NativeEngine` (text or token ids), the reference agent's result. "prefix_ids" come
+    before "ids"."""
     options = {k: v for k, v in payload.items() if k in ALLOWED}
     if "ids" in payload:
-        pieces = list(engine.generate(ids=payload["ids"], reset=True, **options))
+        ids = [*payload.get("prefix_ids", ()), *payload["ids"]]
+        pieces = list(engine.generate(ids=ids, reset=True, **options))
     else:
+        if payload.get("prefix_ids"):
+            raise ValueError("prefix_ids go with ids, not with text")
         pieces = list(engine.generate(text=payload.get("text", ""), reset=True, **options))
     return {"text": "".join(pieces), "tokens": engine.last_tokens, "token_sha256": token_sha256(engine.last_tokens),
             "stats": engine.last, "device": engine.info.get("device")}
@@ -42,9 +46,11 @@ class GreedyExecutor:
     Payload: {"ids": [...], "max_new_tokens": n}. Prefill, then the device decode loop (argmax fed
     back on the GPU); one host sync per request, to read the first token. A grouped lease,
     {"batch": [payload, ...]}, runs its requests together (`batch.generate_batch`: one batched pass
-    per decode step for all of them) and answers {"batch": [result, ...]}; with "prefix_ids" beside "batch"
-    every request's ids follow that prefix, which is run and kept once (`batch.generate_shared`). Optional
-    `timer` (callable(start: bool)) brackets the device work of each lease."""
+    per decode step for all of them) and answers {"batch": [result, ...]}.
+
+    "prefix_ids" in a payload are token ids before its "ids". With "prefix_ids" beside "batch" (or the same ones
+    in every payload of it) every request's ids follow that prefix, which is run and kept once
+    (`batch.generate_shared`). Optional `timer` (callable(start: bool)) brackets the device work of each lease."""
 
     def __init__(self, engine, capacity: int, timer=None):
         self.engine = engine
@@ -55,9 +61,17 @@ class GreedyExecutor:
 
     def _batch(self, items, prefix=()) -> dict:
         from ..batch import MAX_BATCH, generate_batch, generate_shared
+        heads = [[int(t) for t in it.get("prefix_ids", ())] for it in items]
+        if any(heads):
+            if prefix:
+                raise ValueError("prefix_ids both beside a batch and inside it")
+            if all(h == heads[0] for h in heads):
+                prefix = heads[0]
         prompts, limits = [], []
-        for it in items:
+        for it, head in zip(items, heads):
             ids = [int(t) for t in it["ids"]]
+            if ids and not prefix:
+                ids = head + ids
             n = int(it.get("max_new_tokens", 32))
             if not ids or n < 1:
                 raise ValueError("a request needs prompt ids and max_new_tokens >= 1")
@@ -86,6 +100,7 @@ class GreedyExecutor:
         n = int(payload.get("max_new_tokens", 32))
         if not ids or n < 1:
             raise ValueError("a request needs prompt ids and max_new_tokens >= 1")
+        ids = [int(t) for t in payload.get("prefix_ids", ())] + ids
         if len(ids) + n > self.kv.capacity:
             raise ValueError("request exceeds the agent's KV capacity")
         dev = self.engine.device
