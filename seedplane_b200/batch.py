@@ -81,12 +81,12 @@ def generate_batch(engine, prompts: Sequence[Sequence[int]], max_new_tokens, sto
 
 
 def generate_shared(engine, prefix: Sequence[int], prompts: Sequence[Sequence[int]], max_new_tokens, stop: Iterable[int] = (),
-                    block: int = 16, page_size: int = 64, timer=None) -> List[List[int]]:
+                    block: int = 16, page_size: int = 64, timer=None, group: Optional[int] = None) -> List[List[int]]:
     """`generate_batch` for requests that all start with `prefix`: the same greedy tokens as for the prompts
     prefix + prompt, with the prefix run through the model once and its keys and values kept once, in pages that every
     request reads (the attention of a step reads them once for the whole batch). Arguments as `generate_batch`; each
-    prompt has at least one token."""
-    from .paged import PageBatch
+    prompt has at least one token. `group`: at most so many requests hold pages at a time (None: all of them); the next
+    ones take the pages of those before."""
     n_req = len(prompts)
     if n_req == 0:
         return []
@@ -99,26 +99,51 @@ def generate_shared(engine, prefix: Sequence[int], prompts: Sequence[Sequence[in
         raise ValueError("empty prompt")
     if len(prefix) + max(len(p) + m for p, m in zip(prompts, limits)) > engine.cfg.max_positions:
         raise ValueError("a request exceeds the model's positions")
+    if group is not None and group < 1:
+        raise ValueError("group must be positive")
     stops = {int(s) for s in stop}
-    dev = engine.device
-    int32 = lambda v: torch.tensor(v, dtype=torch.int32).to(dev)  # noqa: E731
+    groups = [slice(b, b + (group or n_req)) for b in range(0, n_req, group or n_req)]
     need = [-(-(len(p) + m) // page_size) for p, m in zip(prompts, limits)]
     n_prefix = -(-len(prefix) // page_size)
-    pages = engine.new_pages(n_prefix + sum(need), page_size)
+    pages = engine.new_pages(n_prefix + max(sum(need[g]) for g in groups), page_size)
+    if timer:
+        timer(True)
+    shared = _run_prefix(engine, pages, prefix, n_prefix)
+    out = []
+    for g in groups:
+        out += _run_group(engine, pages, shared, n_prefix, prompts[g], limits[g], need[g], stops, block)
+    if timer:
+        timer(False)
+    engine.status()
+    return out
+
+
+def _int32(v, dev):
+    return torch.tensor(v, dtype=torch.int32).to(dev)
+
+
+def _run_prefix(engine, pages, prefix, n_prefix) -> dict:
+    """The prefix's keys and values into the first pages, as one request's own keys; how a `PageBatch` names them."""
+    from .paged import PageBatch
+    dev = engine.device
     prefix_table = torch.arange(n_prefix, dtype=torch.int32, device=dev)
+    for c0 in range(0, len(prefix), MAX_PASS_TOKENS):
+        part = prefix[c0:c0 + MAX_PASS_TOKENS]
+        one = PageBatch(prefix_table[None], _int32([c0 + len(part)], dev), max_q=len(part))
+        engine.forward_pages(pages, one, _int32(part, dev))
+    return dict(prefix_table=prefix_table, prefix_len=len(prefix))
+
+
+def _run_group(engine, pages, shared, first_page, prompts, limits, need, stops, block) -> List[List[int]]:
+    """The requests' tokens after a prefix that has been run; their pages (`need` each) start at `first_page`."""
+    from .paged import PageBatch
+    n_req, dev = len(prompts), engine.device
     tables = torch.zeros((n_req, max(need)), dtype=torch.int32)
-    at = n_prefix
+    at = first_page
     for b, m in enumerate(need):
         tables[b, :m] = torch.arange(at, at + m, dtype=torch.int32)
         at += m
     tables = tables.to(dev)
-    if timer:
-        timer(True)
-    for c0 in range(0, len(prefix), MAX_PASS_TOKENS):          # the prefix, as one request's own keys
-        part = prefix[c0:c0 + MAX_PASS_TOKENS]
-        one = PageBatch(prefix_table[None], int32([c0 + len(part)]), max_q=len(part))
-        engine.forward_pages(pages, one, int32(part))
-    shared = dict(prefix_table=prefix_table, prefix_len=len(prefix))
     done_rows, firsts = [0] * n_req, [None] * n_req
     b = 0
     while b < n_req:                                           # prompts packed into passes; a long one in several
@@ -135,9 +160,9 @@ def generate_shared(engine, prefix: Sequence[int], prompts: Sequence[Sequence[in
         starts = [0]
         for _, _, take in rows:
             starts.append(starts[-1] + take)
-        part = PageBatch(tables[rows[0][0]:rows[-1][0] + 1], int32([r0 + take for _, r0, take in rows]), q_start=int32(starts),
+        part = PageBatch(tables[rows[0][0]:rows[-1][0] + 1], _int32([r0 + take for _, r0, take in rows], dev), q_start=_int32(starts, dev),
                          tokens=len(flat), max_q=max(take for _, _, take in rows), **shared)
-        argmax, _ = engine.forward_pages(pages, part, int32(flat))
+        argmax, _ = engine.forward_pages(pages, part, _int32(flat, dev))
         for j, (r, r0, take) in enumerate(rows):
             if r0 + take == len(prompts[r]):
                 firsts[r] = argmax[j]
@@ -148,15 +173,12 @@ def generate_shared(engine, prefix: Sequence[int], prompts: Sequence[Sequence[in
         for c0 in range(0, len(active), MAX_BATCH):
             group = active[c0:c0 + MAX_BATCH]
             n = max(1, min(block, min(limits[b] - len(out[b]) for b in group)))
-            step = PageBatch(tables[int32(group).long()], int32([len(prompts[b]) + len(out[b]) - 1 for b in group]), **shared)
-            rows = engine.decode_pages(pages, step, int32([out[b][-1] for b in group]), n).cpu().tolist()
+            step = PageBatch(tables[_int32(group, dev).long()], _int32([len(prompts[b]) + len(out[b]) - 1 for b in group], dev), **shared)
+            rows = engine.decode_pages(pages, step, _int32([out[b][-1] for b in group], dev), n).cpu().tolist()
             for j, b in enumerate(group):
                 for i in range(n):
                     out[b].append(rows[i][j])
                     if rows[i][j] in stops or len(out[b]) >= limits[b]:
                         done[b] = True
                         break
-    if timer:
-        timer(False)
-    engine.status()
     return out

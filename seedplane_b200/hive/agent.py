@@ -50,7 +50,7 @@ class GreedyExecutor:
 
     "prefix_ids" in a payload are token ids before its "ids". With "prefix_ids" beside "batch" (or the same ones
     in every payload of it) every request's ids follow that prefix, which is run and kept once
-    (`batch.generate_shared`). Optional `timer` (callable(start: bool)) brackets the device work of each lease."""
+    (`batch.generate_shared`). However long a lease, MAX_BATCH requests hold keys at a time. Optional `timer` (callable(start: bool)) brackets the device work of each lease."""
 
     def __init__(self, engine, capacity: int, timer=None):
         self.engine = engine
@@ -80,7 +80,7 @@ class GreedyExecutor:
             prompts.append(ids)
             limits.append(n)
         if prefix:
-            out = generate_shared(self.engine, prefix, prompts, limits, timer=self.timer)
+            out = generate_shared(self.engine, prefix, prompts, limits, timer=self.timer, group=MAX_BATCH)
             dev = str(self.engine.device)
             return {"batch": [{"tokens": t, "token_sha256": token_sha256(t), "device": dev} for t in out]}
         while len(self.batch_kvs) < min(len(items), MAX_BATCH):
