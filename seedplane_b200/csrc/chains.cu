@@ -9,7 +9,7 @@
 //                   152,064).
 //   k_chain_sums    (request, piece of the vocabulary): joins the chunks and walks the chain (every piece's CTA for
 //                   itself: less than a launch), then fp64 sums of the rows that are drawn from. The rows' fp32
-//                   sums decide a draft when u q and p differ by more than the sums may be off (kChainSlack); a
+//                   sums decide a draft when u q and p differ by more than the sums may be off (chain_slack); a
 //                   draft that is nearer (one in 10,000) is summed as if refused and left to k_chain_pick. A draw
 //                   compares a running sum over the vocabulary with a given number, and an fp32 sum of 1e5 terms
 //                   would move the border by more than many tokens' whole probability.
@@ -20,10 +20,11 @@
 // The pieces spread the requests' fp64 work (four exponentials a token after a refusal, else one) over all SMs; a
 // cluster of 8 CTAs per request for the last four took 43 us for 32 requests and 36 for 48 without a drafter, these
 // 40 and 24.
-// How far k_chain_stats' sum may be off, relatively: z = (l - max) / T in base 2 carries four roundings (1 / T has
-// two), so a term is off by 4 2^-24 |z| ln 2, and terms below 2^-60 of the largest weigh nothing: 2^-16.6 at
-// |z| = 60; the exponential 2^-22; the sums over a thread's 64 terms, a warp, a CTA and the chunks at most
-// 92 2^-24: below 2^-15.9 together. u q / p takes two such sums: 2^-14.9.
+// How far k_chain_stats' sum may be off, relatively and in units of 2^-24: z = (l - max) / T in base 2 carries four
+// roundings (1 / T has two), so a term is off by 4 |z| ln 2, and terms below 2^-60 of the largest weigh nothing: 169 at
+// |z| = 60 (the joins' exponents add up to z); the exponential 4; the sums over a thread's 64 terms and a warp 69; a join
+// of two maxima's sums 5, one rounding and a factor's exponential, 3 of them in a CTA, 5 in a warp over the chunks and one
+// for every 32 chunks: 282 + 5 ceil(chunks / 32) (chain_slack). u q / p takes two such sums: 2^-14.8 for 152,064 logits.
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -41,7 +42,8 @@ constexpr int kPieceThreads = 256;
 constexpr int kPieceMost = 4096;             // logits per CTA of k_chain_sums and k_chain_left at most
 constexpr int kBatch = 8;                    // logits a thread has under way
 constexpr int kPickThreads = 512;
-constexpr double kChainSlack = 1.0 / 16384;  // 2^-14, above what two sums may be off
+// above what two sums may be off: 2^-14, and more from 12 million logits on
+inline double chain_slack(int chunks) { return std::max(1.0 / 16384, 2.0 * (282 + 5 * ((chunks + 31) / 32)) / (1 << 24)); }
 
 struct ChainStat {                           // of a chunk or a row
     float sum;                               // sum of exp((l - max) / T)
@@ -212,6 +214,7 @@ struct ChainScratch {
     double *sp, *sq, *left;                  // [B][pieces]
     int piece, pieces;                       // logits of a piece, pieces of a row
     int chunk, chunks;                       // likewise of the statistics
+    double slack;                            // how near u q and p leave a draft undecided, relative to p
 };
 // Pieces of 4,096 logits, or of half while they leave SMs idle: for one request's four drafts 18 against 21 us
 // (a quarter: 20), for 32 requests 88 against 81.
@@ -303,7 +306,7 @@ SP_DEVINL ChainPlan chain_decide(const ChainArgs &a, const ChainScratch &sc, int
                     qx = dq.max > -INFINITY ? weigh(lq, dq.max) / dq.sum : 0.0;
                 }
                 const double uq = u * qx;
-                dec = px == 0.0 ? 0 : fabs(uq - px) <= kChainSlack * px ? 2 : uq < px;
+                dec = px == 0.0 ? 0 : fabs(uq - px) <= sc.slack * px ? 2 : uq < px;
             }
         }
         s_dec[tid] = dec;
@@ -661,6 +664,7 @@ ChainScratch chain_scratch(const ChainArgs &a, void *base) {
     ChainScratch sc{};
     sc.chunk = chain_chunk(a.B * (2 * a.n + 1), a.V);
     sc.chunks = (a.V + sc.chunk - 1) / sc.chunk;
+    sc.slack = chain_slack(sc.chunks);
     sc.piece = chain_piece(a.B, a.V);
     sc.pieces = (a.V + sc.piece - 1) / sc.piece;
     const size_t pieces = (size_t)a.B * sc.pieces * sizeof(double);
