@@ -256,6 +256,58 @@ def batch_steps(eng, B: int, repeat: int) -> dict:
     return res
 
 
+def shared_steps(eng, B: int, keys: int, repeat: int) -> dict:
+    """B requests that share `keys` keys: device milliseconds per greedy step over `repeat` steps, each request with a
+    cache of its own (sp_decode_batch) and all of them over the prefix's pages (sp_decode_pages), and whether both gave
+    the same tokens."""
+    from .batch import MAX_PASS_TOKENS
+    from .paged import PageBatch
+    prompt = list(map(int, random_prompt(eng.cfg.vocab, keys, seed=0)))
+    first = [int(t) for t in random_prompt(eng.cfg.vocab, B, seed=1)]
+    warm, dev = 3, eng.device
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+
+    def timed(step):                                          # step(n): n more steps, tokens int32 [n][B]
+        out = [step(warm)]
+        torch.cuda.synchronize()
+        s, e = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        s.record()
+        out.append(step(repeat))
+        e.record()
+        torch.cuda.synchronize()
+        return s.elapsed_time(e) / repeat, torch.cat(out).cpu()
+
+    kvs = [eng.new_kv(keys + warm + repeat + 8) for _ in range(B)]
+    eng.prefill_batch(kvs[:1], [prompt])
+    for kv in kvs[1:]:
+        eng.kv_copy(kvs[0], 0, kv, 0, keys)
+        kv.length = keys
+    state = {"tokens": first, "pos": keys}
+
+    def separate(n):
+        out = eng.decode_batch(kvs, state["tokens"], [state["pos"]] * B, n)
+        state.update(tokens=out[-1].cpu().tolist(), pos=state["pos"] + n)
+        return out
+
+    own_ms, own = timed(separate)
+    for kv in kvs:
+        kv.close()
+    page, each = 64, -(-(warm + repeat + 1) // 64)
+    n_prefix = -(-keys // page)
+    pages = eng.new_pages(n_prefix + B * each, page)
+    prefix_table = torch.arange(n_prefix, dtype=torch.int32, device=dev)
+    for c0 in range(0, keys, MAX_PASS_TOKENS):
+        part = prompt[c0:c0 + MAX_PASS_TOKENS]
+        eng.forward_pages(pages, PageBatch(prefix_table[None], i32([c0 + len(part)]), max_q=len(part)), i32(part))
+    tables = torch.arange(n_prefix, n_prefix + B * each, dtype=torch.int32, device=dev).view(B, each)
+    batch = PageBatch(tables, torch.zeros(B, dtype=torch.int32, device=dev), prefix_table=prefix_table, prefix_len=keys)
+    tokens = i32(first)
+    shared_ms, shared = timed(lambda n: eng.decode_pages(pages, batch, tokens, n))
+    eng.status()
+    return {"model": eng.cfg.name, "requests": B, "shared_keys": keys, "separate_step_ms": own_ms, "pages_step_ms": shared_ms,
+            "tokens_equal": bool(torch.equal(own, shared))}
+
+
 def prompt_passes(eng, prompt, repeat: int, capacity: int) -> dict:
     """Prompt passes (device milliseconds per pass over `repeat` passes), then one more inside the
     profiler range."""
@@ -334,10 +386,13 @@ def main():
     ap.add_argument("--prefill-pass", action="store_true",
                     help="instead of decoding: `--repeat` + 1 prompt passes of `--prompt` tokens (the batched pass, "
                          "last token's head only); the last runs between cudaProfilerStart / Stop")
-    ap.add_argument("--batch", type=int, default=0,
+    ap.add_argument("--batch", default="0",
                     help="instead of decoding one request: this many requests (prompts of 32..128 tokens, packed "
                          "into batched passes), then `--repeat` batched decode steps (sp_decode_batch) and one more "
                          "between cudaProfilerStart / Stop")
+    ap.add_argument("--shared-keys", default="",
+                    help="with --batch (a comma list here): requests that share this many keys (a comma list), steps over "
+                         "caches of their own against steps over the prefix's pages (sp_decode_pages)")
     ap.add_argument("--sampling", type=int, default=0,
                     help="instead of decoding: the device sampling path of a stochastic speculative round with a tree "
                          "of this many nodes at the model's vocabulary (seeded random logits): `--repeat` rounds "
@@ -359,8 +414,15 @@ def main():
     if a.verify:
         print(json.dumps(verify_passes(CudaQwen2(cfg, w, weight_format=fmt), prompt, a.verify, a.repeat, a.capacity)))
         return
-    if a.batch:
-        print(json.dumps(batch_steps(CudaQwen2(cfg, w, weight_format=fmt), a.batch, a.repeat)))
+    batches = [int(b) for b in a.batch.split(",")]
+    if a.shared_keys:
+        eng = CudaQwen2(cfg, w, weight_format=fmt)
+        for keys in a.shared_keys.split(","):
+            for b in batches:
+                print(json.dumps(shared_steps(eng, b, int(keys), a.repeat)))
+        return
+    if batches[0]:
+        print(json.dumps(batch_steps(CudaQwen2(cfg, w, weight_format=fmt), batches[0], a.repeat)))
         return
     if a.prefill_pass:
         print(json.dumps(prompt_passes(CudaQwen2(cfg, w, weight_format=fmt), prompt, a.repeat, a.capacity)))
