@@ -288,10 +288,14 @@ int64_t sp_pages_attention_workspace(const sp_pages *pages, const sp_page_batch 
  * prefix's keys and the request's own keys up to the row's own; the prefix's pages are read once for
  * the whole batch. q, out: [row][heads * head_dim], q_stride / out_stride elements apart (multiples of
  * 8, 16-byte aligned). dtype of q and out: SP_F32 over SP_F16 pages (scores and values then carry the
- * queries and probabilities as two fp16 halves: 2^-22 of each, and of a query 2^-39 of its row's largest), or the pages' own type (probabilities
- * rounded to it; sums, maxima and outputs fp32, rounded once). Over SP_F16 pages a probability is off by
- * 2^-36 (fp32 queries) or 2^-32 of the row's largest besides, fp16's least steps. A row that sees no key gives zeros. Slots that
- * hold no key may hold anything; the values of keys that another row of the request sees must be finite.
+ * queries and probabilities as two fp16 halves: 2^-22 of each, and of a query 2^-39 of its row's
+ * largest), or the pages' own type (probabilities rounded to it; sums, maxima and outputs fp32, rounded
+ * once). Over SP_F16 pages a probability is off by 2^-36 (fp32 queries) or 2^-32 of the row's largest
+ * besides, fp16's least steps. q . K must stay within fp32's range. fp32 queries: the products'
+ * accumulators cut off 2^-23 of a sum for 16 keys at most, over ranges of 4,096 keys; a prefix (or a
+ * request) of more than 131,072 keys is cut into 32 ranges, and the error grows with them. A row that
+ * sees no key gives zeros. Slots that hold no key may hold anything; the values of keys that another row
+ * of the request sees must be finite.
  * lse_dev: NULL or fp32 [row][heads], the log-sum-exp of the scaled scores (-inf for such a row).
  * workspace_dev: as many bytes as sp_pages_attention_workspace says, 16-byte aligned, contents free,
  * not shared by calls that may overlap in time. Can be captured into a graph. */
@@ -336,8 +340,9 @@ int64_t sp_accept_chains_workspace(int32_t batch, int32_t drafts, int32_t vocab)
  * target_dev: [b][drafts + 1][vocab], rows target_ld and requests target_bs elements apart; draft_dev:
  * [b][drafts][vocab], draft_ld, draft_bs; dtype SP_F32, SP_F16 or SP_BF16; u_dev fp64 [b][drafts + 1] in
  * [0, 1). out_tokens_dev int32 [b][drafts + 1]: the accepted tokens, the drawn one, then -1;
- * accepted_dev int32 [b]. drafts 0 .. 64 (0: a draw for every request). Probabilities and sums are
- * fp64. workspace_dev as above. */
+ * accepted_dev int32 [b]. drafts 0 .. 64 (0: a draw for every request). What is decided is decided in fp64: the
+ * fp32 sums of the one pass over the logits settle only the drafts that they cannot be wrong about. workspace_dev as
+ * above. */
 int sp_accept_chains(int device, int32_t batch, int32_t drafts, int32_t vocab, const void *target_dev, int64_t target_bs,
                      int64_t target_ld, const void *draft_dev, int64_t draft_bs, int64_t draft_ld, int32_t dtype,
                      const int32_t *tokens_dev, const int32_t *counts_dev, const double *u_dev,

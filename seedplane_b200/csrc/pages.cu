@@ -805,7 +805,8 @@ PagesPlan plan_attention(const PagesAttention &p) {
         pl.slots = 1;
         return pl;
     }
-    // key ranges that fill the GPU; fp32 queries: no longer than `most` (what the MMAs' accumulators cut off)
+    // key ranges that fill the GPU; fp32 queries: no longer than `most` (what the MMAs' accumulators cut off), up to
+    // kPagesMaxSplits ranges
     const auto splits = [&](long long ctas, long long want, long long keys, long long most) {
         const long long least = f32 ? up(keys, most) : 1;
         return std::min<long long>({std::max<long long>(least, want / ctas), up(keys, kPagesOwnKeys), kPagesMaxSplits});
