@@ -15,8 +15,8 @@
 //                   would move the border by more than many tokens' whole probability.
 //   k_chain_left    (request, piece): fp64 sums of max(p - q, 0), for requests with a refused draft and a drafter
 //   k_chain_pick    a CTA per request: the piece and in it the index whose running sum passes u times the total
-// For 32 requests' five drafts, 152,064 logits, each alone and cold: 36, 26, 19 and 12 us; together 76, at a floor of
-// 32.7 (0.214 GB once, 6.5 TB/s). k_chain_stats runs at 5.9 TB/s; the others are short and wait for one another.
+// For 32 requests' five drafts, 152,064 logits, each alone and cold: 37, 27, 20 and 13 us; together 77, at a floor of
+// 32.7 (0.214 GB once, 6.5 TB/s). k_chain_stats runs at 5.7 TB/s; the others are short and wait for one another.
 // The pieces spread the requests' fp64 work (four exponentials a token after a refusal, else one) over all SMs; a
 // cluster of 8 CTAs per request for the last four took 43 us for 32 requests and 36 for 48 without a drafter, these
 // 40 and 24.

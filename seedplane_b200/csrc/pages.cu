@@ -244,8 +244,8 @@ cudaError_t append_typed(const PagesAppend &p, cudaStream_t s) {
 // private ring of shared memory (cp.async, two tiles deep: three CTAs a SM; no block barrier in the loop) and
 // keeps its own (m, l, O); the warps' results are joined at the end, the key ranges' by
 // k_pages_merge. 64 requests' own keys (35,484 x 4 heads of 128, 73 MB) alone and cold: 24 us (3.0
-// TB/s: 257 x 4 CTAs of unequal lengths); two tiles deep at three CTAs a SM beat three tiles at two (41 -> 39 us with
-// the prefix beside it).
+// TB/s: 257 x 4 CTAs of unequal lengths), with the prefix beside it and the join 37.5; two tiles deep at three CTAs a SM
+// beat three tiles at two (by 2 us).
 constexpr int kRowsWarps = 4, kRowsStages = 2;
 constexpr int kRowsTileBytes = 4096;                         // K (or V) rows of one warp's tile
 // Probabilities are held times 2^kRowsBias: at most 2^14, and what fp16's subnormals round off is 2^-39 of the maximum's
@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 3) k_pages_rows(PagesAttentio
             mt[i] = fmaxf(mt[i], __shfl_xor_sync(0xffffffffu, mt[i], 2));
             const float mn = fmaxf(m[i], mt[i]);
             ms[i] = mn == -INFINITY ? 0.f : mn;              // a row that has seen no key yet
-            corr[i] = max_factor(m[i], mn, sc);
+            corr[i] = exp2_approx((m[i] - ms[i]) * sc);
             m[i] = mn;
             l[i] *= corr[i];
         }

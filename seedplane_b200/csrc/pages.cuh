@@ -56,8 +56,6 @@ SP_DEVINL float row_lse(float m, float l, float c) {
     return l == 0.f ? -INFINITY : fmaf(m, c, log2f(l)) * 0.6931471805599453f;
 }
 SP_DEVINL float row_scale(const PagesAttention &p) { return p.scale * 1.4426950408889634f; }
-// 2^((a - b) c) of two maxima a <= b, -inf where there was no key: 1 for none at all
-SP_DEVINL float max_factor(float a, float b, float c) { return b == -INFINITY ? 1.f : exp2_approx((a - b) * c); }
 
 // fp32 queries are split into fp16 halves after a power of two, exact to take back, that brings the row's largest |q| into
 // [2^14, 2^15): any finite query has halves then, and what the lo half rounds off is 2^-39 of the largest

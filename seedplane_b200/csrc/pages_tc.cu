@@ -8,8 +8,9 @@
 //         queries), so that the sums and O seldom need rescaling (P <= 2^15 then, within either 16-bit type's range);
 //         written over S_q in TMEM in the cache's type
 //   O_q += P_q V     tcgen05.mma with A = P_q in TMEM, B = V as it lies in its pages (MN-major)
-// Packed prompts (12 requests, 3,679 rows x 28 heads over 3,001 + 560 keys) take 195 us, 917 TFLOP/s, at the 1,000 W
-// cap (1.8 GHz); the MMAs alone take 127 us, with the tiles' loads 151, the softmax with the loads 176. A row tile's
+// Packed prompts (12 requests, 3,679 rows x 28 heads over 3,001 + 560 keys) take 199 us, 898 TFLOP/s, at the 1,000 W
+// cap (1.8 GHz); the MMAs alone take 127 us, with the tiles' loads 151, the softmax with the loads 176 (before the
+// exponents took their differences first, 2.5 us in all). A row tile's
 // steps follow one another, so two row tiles take turns:
 //   warps 0-7, 8-15  one row tile each, two threads a row with 64 columns each: tcgen05.ld of the scores, maximum,
 //                    exponentials (in fp32, base 2), tcgen05.st in place (one thread a row and 128 registers of
@@ -49,7 +50,7 @@ constexpr int kTcFlush = 2;                  // fp32 queries: O is added up in f
 // they end at 2^15, and its subnormals' rounding, 2^-25, lies kTcBias further below the maximum: without
 // it many small weights behind a large one (a key that takes most of the weight and has a value near 0) lose their bits.
 // A shorter lag means a longer bias and more rescaling: none for fp16 queries (prompts 196 us, with a lag of 4 207), but
-// fp32 ones carry a lo half too (prompts 465 us with a lag of 8, 481 with 4, 490 with 2). bf16 has fp32's range.
+// fp32 ones carry a lo half too (3,679 rows 465 us with a lag of 8, 481 with 4, 490 with 2). bf16 has fp32's range.
 template <typename TQ, typename TC>
 constexpr float kTcGrow = std::is_same<TC, __half>::value && sizeof(TQ) == 4 ? 4.0f : 8.0f;
 template <typename TQ, typename TC>
@@ -524,7 +525,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const bool flush = kSplit && !alt && i > 0 && i % kTcFlush == 0;
                 if (any && (flush || __any_sync(0xffffffffu, grow))) {
                     // s_full of this tile came after the products of the tile before: O is at rest
-                    const float f = grow ? max_factor(m, mt, c) : 1.f;
+                    const float f = grow ? exp2_approx((m - mt) * c) : 1.f;
                     l *= f;
 #pragma unroll 1
                     for (int k = 0; k < HD / 32; ++k) {

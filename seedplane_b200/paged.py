@@ -151,7 +151,7 @@ def append(pages: PagedKV, layer: int, batch: PageBatch, qkv: torch.Tensor, head
     * head_dim] in the fused q | k | v order, plus `bias` (fp32); the first rot_dim dims of every q and k
     head rotated by `rope` (fp32 [positions, rot_dim / 2, 2] of cos, sin; `engine.rope_table`'s layout) at
     `positions` (int32 [tokens]; None: prefix_len + own key). Returns q [tokens, heads, head_dim] in
-    qkv's type."""
+    qkv's type (fp32 rows into bf16 pages: round it to bf16 for `attention`)."""
     hd = pages.head_dim
     batch._check(pages, layer)
     cols = (heads + 2 * pages.kv_heads) * hd
