@@ -335,8 +335,9 @@ int64_t sp_accept_chains_workspace(int32_t batch, int32_t drafts, int32_t vocab)
  * first refusal i the next token is drawn from max(p_i - q_i, 0), or from p_i where that is zero
  * everywhere; after n acceptances from p_n. A draw from weights r is the first index whose running
  * sum exceeds u[b][drafts] * (their sum). T_b = temperature_dev[b] (fp32; NULL: 1); T_b <= 0 or NaN: greedy,
- * p_i is 1 at the row's first maximum. NaN logits weigh nothing, nor do those below 2^-1000 of the row's largest; a row without a finite or +inf logit
- * accepts nothing and draws -1; a drafted token outside [0, vocab) is refused.
+ * p_i is 1 at the row's first maximum. NaN logits weigh nothing, nor do those below 2^-1000 of the row's
+ * largest; a row without a finite or +inf logit accepts nothing and draws -1; a drafted token outside [0, vocab)
+ * is refused.
  * target_dev: [b][drafts + 1][vocab], rows target_ld and requests target_bs elements apart; draft_dev:
  * [b][drafts][vocab], draft_ld, draft_bs; dtype SP_F32, SP_F16 or SP_BF16; u_dev fp64 [b][drafts + 1] in
  * [0, 1). out_tokens_dev int32 [b][drafts + 1]: the accepted tokens, the drawn one, then -1;

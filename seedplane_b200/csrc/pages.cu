@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 3) k_pages_rows(PagesAttentio
     }
     // own keys each row sees: below this
     const int sa = own0 + ra / G + 1, sb = own0 + rb / G + 1;
-    const float sc = row_scale(p) * up;
+    const float sc = kSplit ? row_scale(p, up) : row_scale(p);
     float o[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;

@@ -3,6 +3,7 @@
 #pragma once
 
 #include <atomic>
+#include <cfloat>
 #include <type_traits>
 
 #include <cuda_bf16.h>
@@ -55,7 +56,10 @@ SP_DEVINL float exp2_approx(float x) {                       // 2^x, relative er
 SP_DEVINL float row_lse(float m, float l, float c) {
     return l == 0.f ? -INFINITY : fmaf(m, c, log2f(l)) * 0.6931471805599453f;
 }
-SP_DEVINL float row_scale(const PagesAttention &p) { return p.scale * 1.4426950408889634f; }
+SP_DEVINL float row_scale(const PagesAttention &p) { return fminf(p.scale * 1.4426950408889634f, FLT_MAX); }
+// c of a row whose queries were divided by `up`: never 0 or infinite (times -inf, or times 0 at the maximum, NaN). The
+// divided row's scores are below 2^40, so that the least normal number leaves nothing of them
+SP_DEVINL float row_scale(const PagesAttention &p, float up) { return fminf(fmaxf(row_scale(p) * up, FLT_MIN), FLT_MAX); }
 
 // fp32 queries are split into fp16 halves after a power of two, exact to take back, that brings the row's largest |q| into
 // [2^14, 2^15): any finite query has halves then, and what the lo half rounds off is 2^-39 of the largest

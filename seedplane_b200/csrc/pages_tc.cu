@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int seen = live ? own0 + row / G + 1 : 0;  // own keys this row sees: below this
             const uint32_t lanes = (uint32_t)(warp & 3) * 32u << 16;
             const uint32_t ts = tmem + lanes + 128u * grp, to = tmem + lanes + 256u + 128u * grp;
-            const float up = kSplit && n > 0 ? s_up[r % (kSplit ? kTcRows : 1)] : 1.f, c = row_scale(p) * up;
+            const float up = kSplit && n > 0 ? s_up[r % (kSplit ? kTcRows : 1)] : 1.f, c = kSplit ? row_scale(p, up) : row_scale(p);
             float m = -INFINITY, l = 0.f;
             uint32_t ph = 0u;
             bool ok = true, any = false, flushed = false;

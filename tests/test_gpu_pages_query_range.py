@@ -58,3 +58,18 @@ def test_rows_of_different_sizes(q, lens, prefix, nh, nkv, hd):
     x[:, 1, ::2] *= 2.0 ** 20
     s["k"][:, :, 0, :, ::2] *= 2.0 ** -20                # head 1's kv head
     check(s, x, hd ** -0.5)
+
+
+@pytest.mark.parametrize("q,lens,prefix,nh,nkv,hd", SHAPES)
+def test_rows_whose_scores_vanish_beside_others(q, lens, prefix, nh, nkv, hd):
+    """A scale for queries of 1e30, and rows of nothing or of 1e-30: every key they see weighs alike."""
+    s = oracle.make_batch(q=q, lens=lens, prefix=prefix, page=64, nkv=nkv, hd=hd, dtype=F16)
+    g = torch.Generator("cuda").manual_seed(7)
+    x = 1e30 * torch.randn(s["rows"], nh, hd, device="cuda", generator=g)
+    x[:, 0] = 0
+    x[:, 1] *= 1e-30
+    x[:, 1] *= 1e-30
+    x[:, 2] = torch.finfo(F32).smallest_normal / 4
+    check(s, x, float(torch.tensor(hd ** -0.5 / 1e30, dtype=F32)))
+    check(s, x * 0, float(torch.finfo(F32).smallest_normal / 8))
+    check(s, x * 0, 3e38)                                # and nothing by the largest scale
