@@ -30,7 +30,7 @@ def native_generate(engine, payload: dict) -> dict:
     before "ids"."""
     options = {k: v for k, v in payload.items() if k in ALLOWED}
     if "ids" in payload:
-        ids = [*payload.get("prefix_ids", ()), *payload["ids"]]
+        ids = [*payload.get("prefix_ids") or (), *payload["ids"]]
         pieces = list(engine.generate(ids=ids, reset=True, **options))
     else:
         if payload.get("prefix_ids"):
@@ -61,7 +61,7 @@ class GreedyExecutor:
 
     def _batch(self, items, prefix=()) -> dict:
         from ..batch import MAX_BATCH, generate_batch, generate_shared
-        heads = [[int(t) for t in it.get("prefix_ids", ())] for it in items]
+        heads = [[int(t) for t in it.get("prefix_ids") or ()] for it in items]
         if any(heads):
             if prefix:
                 raise ValueError("prefix_ids both beside a batch and inside it")
@@ -95,12 +95,12 @@ class GreedyExecutor:
     def __call__(self, payload: dict) -> dict:
         import torch
         if "batch" in payload:
-            return self._batch(payload["batch"], [int(t) for t in payload.get("prefix_ids", ())])
+            return self._batch(payload["batch"], [int(t) for t in payload.get("prefix_ids") or ()])
         ids = [int(t) for t in payload["ids"]]
         n = int(payload.get("max_new_tokens", 32))
         if not ids or n < 1:
             raise ValueError("a request needs prompt ids and max_new_tokens >= 1")
-        ids = [int(t) for t in payload.get("prefix_ids", ())] + ids
+        ids = [int(t) for t in payload.get("prefix_ids") or ()] + ids
         if len(ids) + n > self.kv.capacity:
             raise ValueError("request exceeds the agent's KV capacity")
         dev = self.engine.device

@@ -119,3 +119,10 @@ def test_native_requests_follow_their_prefix():
     assert eng.got["ids"] == [3]
     with pytest.raises(ValueError):
         native_generate(eng, {"text": "a", "prefix_ids": [1]})
+
+
+def test_no_prefix_by_any_name(executor):
+    plain = executor({"ids": [5, 6], "max_new_tokens": 2})
+    assert executor({"ids": [5, 6], "prefix_ids": None, "max_new_tokens": 2}) == plain
+    batch_of = {"batch": [{"ids": [4], "prefix_ids": None, "max_new_tokens": 1}], "prefix_ids": None}
+    assert tokens(executor(batch_of)) == [[4]]
