@@ -30,7 +30,7 @@ def native_generate(engine, payload: dict) -> dict:
     before "ids"."""
     options = {k: v for k, v in payload.items() if k in ALLOWED}
     if "ids" in payload:
-        ids = [*payload.get("prefix_ids") or (), *payload["ids"]]
+        ids = [*(payload.get("prefix_ids") or ()), *payload["ids"]]
         pieces = list(engine.generate(ids=ids, reset=True, **options))
     else:
         if payload.get("prefix_ids"):
